@@ -125,6 +125,14 @@ SIGNATURES: dict[str, tuple] = {
         [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _P, _I32,
          ctypes.POINTER(AdamHParams), _TUNE, _P],
     ),
+    "axon_adam_scaled": (
+        _I32,
+        [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _P, _I32, _P,
+         ctypes.POINTER(AdamHParams), _TUNE, _P],
+    ),
+    "axon_grad_norm_workspace_bytes": (_I64, [_I64]),
+    "axon_grad_norm": (_I32, [_P, _P, _P, _I64, _F, _F, _P, _P, _P, _I64, _P]),
+    "axon_clip_grads": (_I32, [_P, _P, _P, _P, _I64, _F, _F, _P, _P, _I64, _P]),
     "axon_gemm": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _TUNE, _P]),
     "axon_gemm_status": (_I32, [_P]),
     "axon_cast": (_I32, [_P, _P, _I64, _I32, _I32, _P]),

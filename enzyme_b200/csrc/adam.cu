@@ -5,7 +5,8 @@
 // order. A grid-stride loop over 8-element groups: each group is one or two
 // 16-byte packets per tensor (fp32 state: 2, bf16 state: 1), read once with
 // evict-first hints and written once -- 26 bytes per parameter for fp32 state
-// with bf16 gradients, HBM-bound.
+// with bf16 gradients, HBM-bound. SCALED multiplies the gradients by a device
+// scalar first (a clip scale; the product is rounded to fp32 before it is used).
 #include "common.cuh"
 
 namespace axon {
@@ -24,6 +25,7 @@ struct AdamArgs {
   const void* ss_rows;
   const void* ib_rows;
   const void* wd_rows;
+  const float* gscale;  // device scalar the gradients are multiplied by, or NULL
   int32_t row_dtype;
   int64_t cols;
   int64_t n;
@@ -75,12 +77,13 @@ __device__ __forceinline__ void row_scalars(const AdamArgs& a, int64_t idx, floa
 
 // Vector path: n % 8 == 0, cols % 8 == 0 (a group never straddles a row), all
 // tensors 16-byte aligned.
-template <typename TS, typename TG>
+template <typename TS, typename TG, bool SCALED>
 __global__ void __launch_bounds__(256) adam_vec(AdamArgs a) {
   const int64_t groups = a.n / G;
   const bool per_row = a.ss_rows || a.ib_rows || a.wd_rows;
   pdl_wait();
   pdl_trigger();
+  const float gscale = SCALED ? *a.gscale : 1.0f;
   for (int64_t gi = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; gi < groups;
        gi += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t off = gi * G;
@@ -92,19 +95,21 @@ __global__ void __launch_bounds__(256) adam_vec(AdamArgs a) {
     float ss = a.ss, ib = a.ib, wd = a.wd;
     if (per_row) row_scalars(a, off, ss, ib, wd);
 #pragma unroll
-    for (int e = 0; e < G; ++e) adam_one(a, ss, ib, wd, p[e], g[e], m[e], v[e]);
+    for (int e = 0; e < G; ++e) adam_one(a, ss, ib, wd, p[e], SCALED ? __fmul_rn(g[e], gscale) : g[e], m[e], v[e]);
     st8(static_cast<TS*>(a.po) + off, p);
     st8(static_cast<TS*>(a.mo) + off, m);
     st8(static_cast<TS*>(a.vo) + off, v);
   }
 }
 
-template <typename TS, typename TG>
+template <typename TS, typename TG, bool SCALED>
 __global__ void adam_scalar(AdamArgs a) {
+  const float gscale = SCALED ? *a.gscale : 1.0f;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < a.n;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     float p = to_f(static_cast<const TS*>(a.p)[i]);
     float g = to_f(static_cast<const TG*>(a.g)[i]);
+    if (SCALED) g = __fmul_rn(g, gscale);
     float m = to_f(static_cast<const TS*>(a.m)[i]);
     float v = to_f(static_cast<const TS*>(a.v)[i]);
     float ss, ib, wd;
@@ -116,7 +121,7 @@ __global__ void adam_scalar(AdamArgs a) {
   }
 }
 
-template <typename TS, typename TG>
+template <typename TS, typename TG, bool SCALED>
 int launch_adam(const AdamArgs& a, int threads, cudaStream_t s) {
   const bool vec = a.n % G == 0 && a.cols % G == 0 && aligned16(a.p) && aligned16(a.g) && aligned16(a.m) &&
                    aligned16(a.v) && aligned16(a.po) && aligned16(a.mo) && aligned16(a.vo);
@@ -126,18 +131,23 @@ int launch_adam(const AdamArgs& a, int threads, cudaStream_t s) {
   if (grid > cap) grid = cap;
   if (grid < 1) grid = 1;
   if (vec)
-    launch_k(adam_vec<TS, TG>, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, a);
+    launch_k(adam_vec<TS, TG, SCALED>, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, a);
   else
-    adam_scalar<TS, TG><<<static_cast<int>(grid), threads, 0, s>>>(a);
+    adam_scalar<TS, TG, SCALED><<<static_cast<int>(grid), threads, 0, s>>>(a);
   return launch_status("axon_adam");
+}
+
+template <typename TS, typename TG>
+int launch_adam_scaled(const AdamArgs& a, int threads, cudaStream_t s) {
+  return a.gscale ? launch_adam<TS, TG, true>(a, threads, s) : launch_adam<TS, TG, false>(a, threads, s);
 }
 
 template <typename TS>
 int dispatch_grad(const AdamArgs& a, int32_t gdt, int threads, cudaStream_t s) {
   switch (gdt) {
-    case AXON_F32: return launch_adam<TS, float>(a, threads, s);
-    case AXON_BF16: return launch_adam<TS, __nv_bfloat16>(a, threads, s);
-    case AXON_F16: return launch_adam<TS, __half>(a, threads, s);
+    case AXON_F32: return launch_adam_scaled<TS, float>(a, threads, s);
+    case AXON_BF16: return launch_adam_scaled<TS, __nv_bfloat16>(a, threads, s);
+    case AXON_F16: return launch_adam_scaled<TS, __half>(a, threads, s);
     default: return fail(AXON_E_UNSUPPORTED, "axon_adam: unsupported grad dtype %d", gdt);
   }
 }
@@ -152,6 +162,17 @@ extern "C" int axon_adam(const void* param, const void* grad, const void* exp_av
                          int32_t state_dtype, int32_t grad_dtype, const void* step_size_rows,
                          const void* inv_bc2_sqrt_rows, const void* wd_rows, int32_t row_dtype,
                          const axon_adam_hparams_t* hp, const axon_tune_t* tune, void* stream) {
+  return axon_adam_scaled(param, grad, exp_avg, exp_avg_sq, param_out, exp_avg_out, exp_avg_sq_out, rows, cols,
+                          state_dtype, grad_dtype, step_size_rows, inv_bc2_sqrt_rows, wd_rows, row_dtype, nullptr, hp,
+                          tune, stream);
+}
+
+extern "C" int axon_adam_scaled(const void* param, const void* grad, const void* exp_avg, const void* exp_avg_sq,
+                                void* param_out, void* exp_avg_out, void* exp_avg_sq_out, int64_t rows, int64_t cols,
+                                int32_t state_dtype, int32_t grad_dtype, const void* step_size_rows,
+                                const void* inv_bc2_sqrt_rows, const void* wd_rows, int32_t row_dtype,
+                                const float* grad_scale, const axon_adam_hparams_t* hp, const axon_tune_t* tune,
+                                void* stream) {
   axon_tune_t t = tune_or_default(tune);
   if (rows < 0 || cols < 0) return fail(AXON_E_SHAPE, "axon_adam: negative size");
   if (!hp) return fail(AXON_E_ARG, "axon_adam: NULL hyper-parameters");
@@ -167,7 +188,7 @@ extern "C" int axon_adam(const void* param, const void* grad, const void* exp_av
   const int64_t n = rows * cols;
   if (n == 0) return AXON_OK;
   AdamArgs a{param, grad, exp_avg, exp_avg_sq, param_out, exp_avg_out, exp_avg_sq_out,
-             step_size_rows, inv_bc2_sqrt_rows, wd_rows, row_dtype, cols, n,
+             step_size_rows, inv_bc2_sqrt_rows, wd_rows, grad_scale, row_dtype, cols, n,
              hp->beta1, hp->beta2, hp->eps, hp->step_size, hp->inv_bc2_sqrt, hp->wd};
   cudaStream_t s = as_stream(stream);
   switch (state_dtype) {

@@ -7,6 +7,7 @@ status and raises `AxonError` on failure. Nothing here computes on the CPU.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -166,11 +167,16 @@ def cumsum_status(workspace=None) -> None:
 
 
 def adam(param, grad, exp_avg, exp_avg_sq, *, step_size=None, inv_bc2_sqrt=None, wd=None, beta1=0.9,
-         beta2=0.999, eps=1e-8, out=None, tune=None):
+         beta2=0.999, eps=1e-8, grad_scale=None, out=None, tune=None):
     """L2-regularised Adam. step_size / inv_bc2_sqrt / wd are floats or
-    per-row tensors [rows] / [rows, 1]. out = (param_out, m_out, v_out) or None
-    for new tensors; pass the inputs themselves to update in place."""
-    _require_cuda(param, grad, exp_avg, exp_avg_sq)
+    per-row tensors [rows] / [rows, 1]. `grad_scale`, a one-element fp32 tensor
+    on the device (grad_norm_scale's scale), multiplies the gradients first.
+    out = (param_out, m_out, v_out) or None for new tensors; pass the inputs
+    themselves to update in place."""
+    _require_cuda(param, grad, exp_avg, exp_avg_sq, grad_scale)
+    if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
+                                   or grad_scale.device != param.device):
+        raise N.AxonError(N.AXON_E_ARG, "adam: grad_scale must be one fp32 value on the parameters' device")
     for t in (param, grad, exp_avg, exp_avg_sq):
         if not t.is_contiguous() or t.shape != param.shape:
             raise N.AxonError(N.AXON_E_SHAPE, "adam: tensors must be contiguous and the same shape")
@@ -194,10 +200,154 @@ def adam(param, grad, exp_avg, exp_avg_sq, *, step_size=None, inv_bc2_sqrt=None,
             if name == "inv_bc2_sqrt" and v is None:
                 hp.inv_bc2_sqrt = 1.0
             row_ptrs.append(None)
-    check(N.lib().axon_adam(_ptr(param), _ptr(grad), _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(out[0]), _ptr(out[1]),
-                            _ptr(out[2]), rows, cols, dtype_code(param), dtype_code(grad), row_ptrs[0], row_ptrs[1],
-                            row_ptrs[2], row_dt, ctypes.byref(hp), _tune(tune), _stream(param)))
+    check(N.lib().axon_adam_scaled(_ptr(param), _ptr(grad), _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(out[0]),
+                                   _ptr(out[1]), _ptr(out[2]), rows, cols, dtype_code(param), dtype_code(grad),
+                                   row_ptrs[0], row_ptrs[1], row_ptrs[2], row_dt, _ptr(grad_scale),
+                                   ctypes.byref(hp), _tune(tune), _stream(param)))
     return out
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one block of memory, each once (any order of
+    the dimensions)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class GradList:
+    """A list of gradients checked and packed once, for calls that come back
+    with the same tensors every step (an optimizer's gradient buffers).
+
+    `grads` are fp32, bf16 or fp16 CUDA tensors of one device, types mixed as
+    they come, empty ones allowed, each dense in memory (any order of its
+    dimensions). `out`, where clip_grads writes, is None (in place) or a list of
+    tensors that match them in shape, type and strides and overlap nothing else
+    in the two lists. The tensors are held; one whose memory has moved
+    since (`set_`, `.data =`, a storage resize) makes the next call raise."""
+
+    def __init__(self, grads, out=None):
+        self.grads = list(grads)
+        self.out = self.grads if out is None else list(out)
+        if not self.grads:
+            raise N.AxonError(N.AXON_E_SHAPE, "gradient list: empty (no device to work on)")
+        if len(self.out) != len(self.grads):
+            raise N.AxonError(N.AXON_E_SHAPE, "gradient list: out must have a tensor for each gradient")
+        _require_cuda(*self.grads, *self.out)
+        self.device = self.grads[0].device
+        for t, o in zip(self.grads, self.out):
+            if t.device != self.device or o.device != self.device:
+                raise N.AxonError(N.AXON_E_ARG, "gradient list: tensors on more than one device")
+            if not _is_dense(t):
+                raise N.AxonError(N.AXON_E_SHAPE, "gradient list: a gradient is not dense in memory")
+            if o is not t and (o.dtype != t.dtype or o.shape != t.shape or
+                               (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))):
+                raise N.AxonError(N.AXON_E_SHAPE, "gradient list: out must match shape, type and strides")
+        n = len(self.grads)
+        self._where = [t.data_ptr() for t in self.grads]
+        self._where_out = [t.data_ptr() for t in self.out]
+        self._in_ptrs = (ctypes.c_void_p * n)(*self._where)
+        self._out_ptrs = (ctypes.c_void_p * n)(*self._where_out)
+        self._sizes = (ctypes.c_int64 * n)(*(t.numel() for t in self.grads))
+        self._dtypes = (ctypes.c_int32 * n)(*(dtype_code(t) for t in self.grads))
+        self._ws_bytes = 0  # asked of the library with the first call (it needs the device's SM count)
+        self._clippable = None
+
+    def _check_overlap(self) -> None:
+        """Outputs are their own input or memory of their own: anything else
+        would be scaled twice or read after it was written."""
+        spans = []
+        for i, (t, o) in enumerate(zip(self.grads, self.out)):
+            nb = t.numel() * t.element_size()
+            if nb == 0:
+                continue
+            spans.append((self._where_out[i], self._where_out[i] + nb, True))
+            if self._where[i] != self._where_out[i]:
+                spans.append((self._where[i], self._where[i] + nb, False))
+        spans.sort()
+        # sweep: an output must not meet any other span; inputs that are only read may overlap each other
+        end_any = end_out = 0
+        for lo, hi, is_out in spans:
+            if lo < (end_any if is_out else end_out):
+                raise N.AxonError(N.AXON_E_ARG, "gradient list: an output overlaps another tensor of the list")
+            end_any = max(end_any, hi)
+            if is_out:
+                end_out = max(end_out, hi)
+
+    def _ready(self, clip: bool):
+        """(workspace, stream) for a call on this list."""
+        if [t.data_ptr() for t in self.grads] != self._where:
+            raise N.AxonError(N.AXON_E_ARG, "gradient list: a gradient's memory has moved; make a new GradList")
+        if clip:
+            if self.out is not self.grads and [t.data_ptr() for t in self.out] != self._where_out:
+                raise N.AxonError(N.AXON_E_ARG, "gradient list: an output's memory has moved; make a new GradList")
+            if self._clippable is None:
+                self._check_overlap()
+                self._clippable = True
+        if self._ws_bytes == 0:
+            self._ws_bytes = _check_ws_bytes(N.lib().axon_grad_norm_workspace_bytes(len(self.grads)))
+        return torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device), _stream(self.grads[0])
+
+
+def _grad_list(grads, out=None) -> GradList:
+    if isinstance(grads, GradList):
+        if out is not None:
+            raise N.AxonError(N.AXON_E_ARG, "gradient list: a GradList has its own out")
+        return grads
+    return GradList(grads, out=out)
+
+
+def _on_device(device):
+    """Makes `device` current where it is not (kernels are launched, and SMs
+    counted, on the current device)."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def grad_norm_scale(grads, max_norm, *, eps=1e-6):
+    """(norm, scale): the L2 norm over all elements of `grads` (a list of
+    tensors or a GradList) and min(1, max_norm / (norm + eps)), both 0-d fp32
+    tensors on the device; pass the scale to adam(grad_scale=...) to clip
+    without rewriting the gradients. A NaN gradient makes both NaN."""
+    g = _grad_list(grads)
+    with _on_device(g.device):
+        ws, stream = g._ready(clip=False)
+        res = torch.empty(2, dtype=torch.float32, device=g.device)
+        check(N.lib().axon_grad_norm(g._in_ptrs, g._sizes, g._dtypes, len(g.grads), float(max_norm), float(eps),
+                                     res.data_ptr(), res.data_ptr() + 4, ws.data_ptr(), g._ws_bytes, stream))
+    return res[0], res[1]
+
+
+def grad_norm(grads):
+    """The L2 norm over all elements of `grads` (a list of tensors or a
+    GradList) as a 0-d fp32 tensor: squares in fp32, their sum in float64 in a
+    fixed order (the same bits every time)."""
+    g = _grad_list(grads)
+    with _on_device(g.device):
+        ws, stream = g._ready(clip=False)
+        norm = torch.empty((), dtype=torch.float32, device=g.device)
+        check(N.lib().axon_grad_norm(g._in_ptrs, g._sizes, g._dtypes, len(g.grads), 1.0, 0.0, norm.data_ptr(), None,
+                                     ws.data_ptr(), g._ws_bytes, stream))
+    return norm
+
+
+def clip_grads(grads, max_norm, *, eps=1e-6, out=None):
+    """Scales the gradients by min(1, max_norm / (norm + eps)), norm the L2
+    norm over all of them; returns (the scaled tensors, norm). In place by
+    default; `out` (or the GradList's) takes the result elsewhere."""
+    g = _grad_list(grads, out)
+    with _on_device(g.device):
+        ws, stream = g._ready(clip=True)
+        norm = torch.empty((), dtype=torch.float32, device=g.device)
+        check(N.lib().axon_clip_grads(g._in_ptrs, g._out_ptrs, g._sizes, g._dtypes, len(g.grads), float(max_norm),
+                                      float(eps), norm.data_ptr(), ws.data_ptr(), g._ws_bytes, stream))
+    return g.out, norm
 
 
 def gemm(a, b, *, b2=None, row_scale=None, epilogue=N.AXON_EPI_NONE, out=None, out_dtype=None, tune=None):

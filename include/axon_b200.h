@@ -239,6 +239,50 @@ AXON_API int axon_adam(const void* param, const void* grad, const void* exp_avg,
               const void* inv_bc2_sqrt_rows, const void* wd_rows, int32_t row_dtype,
               const axon_adam_hparams_t* hp, const axon_tune_t* tune, void* stream);
 
+/* axon_adam with the gradients multiplied by *grad_scale first (g * scale in
+ * fp32): a device scalar, such as the clip scale axon_grad_norm writes, so
+ * that a clipped step needs no pass that rewrites the gradients.
+ * grad_scale NULL is axon_adam. No counterpart in the reference (its spec takes
+ * gradients as they are). */
+AXON_API int axon_adam_scaled(const void* param, const void* grad, const void* exp_avg,
+              const void* exp_avg_sq, void* param_out, void* exp_avg_out,
+              void* exp_avg_sq_out, int64_t rows, int64_t cols, int32_t state_dtype,
+              int32_t grad_dtype, const void* step_size_rows,
+              const void* inv_bc2_sqrt_rows, const void* wd_rows, int32_t row_dtype,
+              const float* grad_scale, const axon_adam_hparams_t* hp,
+              const axon_tune_t* tune, void* stream);
+
+/* ---- gradient norm and clipping --------------------------------------------------
+ * No counterpart in the reference; the step between a backward pass and
+ * axon_adam. grads, outs, sizes and dtypes are HOST arrays of `count` entries:
+ * device pointers aligned to their element, element counts (0 allowed) and
+ * AXON_F32 / AXON_BF16 / AXON_F16, mixed as they come. They are read before
+ * the call returns. A tensor may start anywhere; 16-byte aligned ones (and,
+ * for clipping, outputs aligned like their inputs) take the fast path.
+ *   norm  = sqrt(sum over all elements of x^2)
+ *   scale = min(1, max_norm / (norm + eps)), 1 where norm + eps is 0
+ * Squares are formed in fp32 (elements beyond 1.8e19 in magnitude make the
+ * norm infinite, below 1e-19 they lose digits) and summed in float64 in a
+ * fixed order: the same list gives the same bits every time. A NaN in any
+ * gradient makes norm and scale NaN, an infinity makes norm infinite and
+ * scale 0 (NaN for an infinite max_norm).
+ * workspace: axon_grad_norm_workspace_bytes(count) bytes for the current
+ * device, 8-byte aligned, uninitialised; calls that may overlap on the GPU
+ * need one each. max_norm and eps are >= 0. */
+AXON_API int64_t axon_grad_norm_workspace_bytes(int64_t count);
+
+/* norm and / or scale (fp32 device scalars; either may be NULL). */
+AXON_API int axon_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes,
+                            int64_t count, float max_norm, float eps, float* norm, float* scale,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* outs[i] = scale * grads[i], of grads[i]'s type and rounded once. outs[i] is
+ * grads[i] (in place; untouched when scale is 1) or memory that overlaps no
+ * grads[j] and no other output. norm may be NULL. */
+AXON_API int axon_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes,
+                             const int32_t* dtypes, int64_t count, float max_norm, float eps,
+                             float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- dense ------------------------------------------------------------------- */
 
 #define AXON_EPI_NONE 0      /* C = A @ B                                        */
