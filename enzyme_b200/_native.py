@@ -34,6 +34,10 @@ AXON_EPI_ROWSCALE = 1
 AXON_EPI_SILU_GATE = 2
 AXON_EPI_EXP = 3
 
+AXON_REDUCE_NONE = 0
+AXON_REDUCE_SUM = 1
+AXON_REDUCE_MEAN = 2
+
 AXON_IPC_HANDLE_BYTES = 64
 
 _CODE_NAMES = {
@@ -135,6 +139,18 @@ SIGNATURES: dict[str, tuple] = {
     "axon_clip_grads": (_I32, [_P, _P, _P, _P, _I64, _F, _F, _P, _P, _I64, _P]),
     "axon_gemm": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _TUNE, _P]),
     "axon_gemm_status": (_I32, [_P]),
+    "axon_linear_ce_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "axon_linear_ce": (
+        _I32,
+        [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I64, _I32, _P, _I64, _TUNE, _P],
+    ),
+    "axon_linear_ce_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _TUNE]),
+    "axon_linear_ce_grad": (
+        _I32,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I64, _I32,
+         _P, _I64, _TUNE, _P],
+    ),
+    "axon_linear_ce_status": (_I32, [_P]),
     "axon_cast": (_I32, [_P, _P, _I64, _I32, _I32, _P]),
     "axon_selftest_bounded_wait": (_I32, [_I64, _P, _P, _P]),
     "axon_row_rsqrt": (_I32, [_P, _P, _I64, _I64, _I64, _I32, _F, _F, _P]),

@@ -519,3 +519,96 @@ def silu_mlp(x, w1, w2, w3, *, out=None, out_dtype=None, workspace=None, tune=No
     check(N.lib().axon_silu_mlp(_ptr(x), _ptr(w1), _ptr(w2), _ptr(w3), _ptr(y), _ptr(ws), ws.numel() * ws.element_size(),
                                 m, n, k, p, dtype_code(x), dtype_code(y), _tune(tune), _stream(x)))
     return y
+
+
+_REDUCE = {"none": N.AXON_REDUCE_NONE, "sum": N.AXON_REDUCE_SUM, "mean": N.AXON_REDUCE_MEAN}
+
+
+def _head_args(name, h, w, targets, reduction):
+    """Checks what the loss and its gradient share; (m, k, v, ld_h, ld_w, target bits, reduction)."""
+    _require_cuda(h, w, targets)
+    m, k, ldh = _rows(h)
+    v, kw, ldw = _rows(w)
+    if kw != k:
+        raise N.AxonError(N.AXON_E_SHAPE, f"{name}: hidden sizes differ ({k} vs {kw})")
+    if w.dtype != h.dtype:
+        raise N.AxonError(N.AXON_E_UNSUPPORTED, f"{name}: h and w must share a type")
+    if targets.shape != (m,) or not targets.is_contiguous():
+        raise N.AxonError(N.AXON_E_SHAPE, f"{name}: targets must be contiguous [{m}]")
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise N.AxonError(N.AXON_E_UNSUPPORTED, f"{name}: targets must be int64 or int32")
+    if w.device != h.device or targets.device != h.device:
+        raise N.AxonError(N.AXON_E_ARG, f"{name}: tensors on more than one device")
+    if reduction not in _REDUCE:
+        raise N.AxonError(N.AXON_E_ARG, f"{name}: reduction must be 'none', 'sum' or 'mean'")
+    if m <= 1:  # the stride of a single row says nothing
+        ldh = max(ldh, k)
+    if v == 1:
+        ldw = max(ldw, k)
+    return m, k, v, ldh, ldw, 8 * targets.element_size(), _REDUCE[reduction]
+
+
+def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", workspace=None, tune=None):
+    """Softmax cross entropy of the logits h @ w.T, which are never stored.
+
+    h [m, k] and w [v, k] (a row per word, as an embedding or nn.Linear holds
+    it) are bf16 or fp16 with k a multiple of 8; targets [m] int64 or int32.
+    Rows whose target is `ignore_index` have loss 0; any other target outside
+    [0, v) gives NaN. Returns (loss, stats): loss the per-row losses ("none"),
+    their sum, or their mean over the rows not ignored, in fp32; stats [2, m]
+    fp32 holds each row's log-sum-exp and loss, for linear_cross_entropy_grad."""
+    m, k, v, ldh, ldw, bits, red = _head_args("linear_cross_entropy", h, w, targets, reduction)
+    stats = torch.empty((2, m), dtype=torch.float32, device=h.device)
+    loss = stats[1] if red == N.AXON_REDUCE_NONE else torch.empty((), dtype=torch.float32, device=h.device)
+    with _on_device(h.device):
+        need = _check_ws_bytes(N.lib().axon_linear_ce_workspace_bytes(m, k, v))
+        ws = _workspace(need, h.device, workspace)
+        check(N.lib().axon_linear_ce(_ptr(h), _ptr(w), _ptr(targets), stats.data_ptr(), stats.data_ptr() + 4 * m,
+                                     loss.data_ptr(), m, k, v, ldh, ldw, dtype_code(h), bits, int(ignore_index), red,
+                                     ws.data_ptr(), ws.numel(), _tune(tune), _stream(h)))
+    return loss, stats
+
+
+def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100, reduction="mean", need=(True, True),
+                              out=None, dw_dtype=None, workspace=None, tune=None):
+    """Gradients of linear_cross_entropy's loss with respect to h and w.
+
+    stats is what the forward call returned, dloss the gradient of its loss:
+    fp32, [m] for "none", one value for "sum" and "mean". Returns (dh, dw), of
+    h's and w's type (dw in fp32 with dw_dtype=torch.float32); need = (True,
+    False) or (False, True) leaves one out (None), out = (dh, dw) names the
+    tensors to write. Rows that are ignored get zeros. tune={"split": words}
+    sets the piece of the vocabulary that is worked on at a time."""
+    name = "linear_cross_entropy_grad"
+    m, k, v, ldh, ldw, bits, red = _head_args(name, h, w, targets, reduction)
+    _require_cuda(stats, dloss)
+    if stats.shape != (2, m) or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.device != h.device:
+        raise N.AxonError(N.AXON_E_ARG, f"{name}: stats must be the forward call's [2, {m}] fp32 tensor")
+    if dloss.dtype != torch.float32 or dloss.device != h.device or not dloss.is_contiguous() or \
+            (dloss.shape != (m,) if red == N.AXON_REDUCE_NONE else dloss.numel() != 1):
+        raise N.AxonError(N.AXON_E_ARG, f"{name}: dloss must be contiguous fp32, "
+                          + (f"[{m}]" if red == N.AXON_REDUCE_NONE else "one value"))
+    if out is not None:
+        dh, dw = out
+    else:
+        dh = torch.empty((m, k), dtype=h.dtype, device=h.device) if need[0] else None
+        dw = torch.empty((v, k), dtype=dw_dtype or w.dtype, device=h.device) if need[1] else None
+    _require_cuda(dh, dw)
+    for t, like, types in ((dh, h, (h.dtype,)), (dw, w, (w.dtype, torch.float32))):
+        if t is not None and (t.shape != like.shape or t.dtype not in types or t.device != h.device):
+            raise N.AxonError(N.AXON_E_ARG, f"{name}: out must have the operands' shapes and types")
+    lddh = max(_rows(dh)[2], k) if dh is not None else 0
+    lddw = max(_rows(dw)[2], k) if dw is not None else 0
+    with _on_device(h.device):
+        nbytes = _check_ws_bytes(N.lib().axon_linear_ce_grad_workspace_bytes(m, k, v, _tune(tune)))
+        ws = _workspace(nbytes, h.device, workspace)
+        check(N.lib().axon_linear_ce_grad(_ptr(h), _ptr(w), _ptr(targets), stats.data_ptr(),
+                                          stats.data_ptr() + 4 * m, _ptr(dloss), _ptr(dh), _ptr(dw), m, k, v, ldh,
+                                          ldw, lddh, lddw, dtype_code(h), dtype_code(dw) if dw is not None else
+                                          dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.numel(),
+                                          _tune(tune), _stream(h)))
+    return dh, dw
+
+
+def linear_cross_entropy_status(device=None) -> None:
+    check(N.lib().axon_linear_ce_status(torch.cuda.current_stream(device).cuda_stream))

@@ -316,6 +316,59 @@ AXON_API int axon_gemm(const void* a, const void* b, const void* b2, void* c,
  * on a bounded pipeline wait (AXON_E_TIMEOUT; the flag is then cleared). */
 AXON_API int axon_gemm_status(void* stream);
 
+/* ---- the output head's loss and its gradient ------------------------------------
+ * No counterpart in the reference; the end of a training step's forward pass
+ * and the start of its backward pass.
+ *   s = h w^T, lse_i = log sum_j exp(s_ij), loss_i = lse_i - s_{i, targets[i]}
+ * h [m, k] (ld_h) and w [v, k] (ld_w: a row per word, the embedding's order),
+ * both AXON_BF16 or both AXON_F16; fp32 accumulation; the logits s are never
+ * stored. k a multiple of 8, leading dimensions multiples of 8, bases 16-byte
+ * aligned; any m (0 too) and v. targets: 32- or 64-bit integers (target_bits);
+ * a row whose target is ignore_index has loss 0 and adds nothing to any
+ * gradient, whatever it holds; any other target outside [0, v) makes its
+ * row's loss, and the gradients, NaN. */
+#define AXON_REDUCE_NONE 0
+#define AXON_REDUCE_SUM 1
+#define AXON_REDUCE_MEAN 2  /* over the rows not ignored; NaN if there is none */
+
+/* lse, loss_rows: fp32 [m] (lse of ignored rows too). loss: one fp32 value for
+ * AXON_REDUCE_SUM / MEAN (summed in float64 in a fixed order), else unused.
+ * loss_rows keeps its relative precision down to losses far below the
+ * logits' rounding: log1p(exp(log-sum-exp of the other words - s_target)).
+ * workspace: axon_linear_ce_workspace_bytes, 16-byte aligned, uninitialised; calls
+ * that may overlap need one each. tune->max_ctas caps the grid. */
+AXON_API int64_t axon_linear_ce_workspace_bytes(int64_t m, int64_t k, int64_t v);
+AXON_API int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse,
+                            float* loss_rows, float* loss, int64_t m, int64_t k, int64_t v,
+                            int64_t ld_h, int64_t ld_w, int32_t dtype, int32_t target_bits,
+                            int64_t ignore_index, int32_t reduction, void* workspace,
+                            int64_t workspace_bytes, const axon_tune_t* tune, void* stream);
+
+/* Gradients for the same operands: with g_i = dloss[i] (AXON_REDUCE_NONE),
+ * dloss[0] (SUM) or dloss[0] / counted rows (MEAN), dloss fp32 on the device,
+ *   d_ij = g_i (exp(s_ij - lse_i) - [j = targets[i]]), dh = d w, dw = d^T h.
+ * lse and loss_rows are axon_linear_ce's. dh [m, k] (ld_dh) has h's type, dw
+ * [v, k] (ld_dw) w's or AXON_F32; either may be NULL. Both are overwritten.
+ * The logits are formed again, a piece of the vocabulary at a time:
+ * tune->split words a piece (a multiple of 256; 0: as many as keep the
+ * piece's d, 16-bit [m, piece], within 512 MB). d is rounded to the operand
+ * type (f16: times a power of two chosen from dloss), and contracted in fp32.
+ * workspace: axon_linear_ce_grad_workspace_bytes (same tune), 256-byte aligned,
+ * uninitialised. */
+AXON_API int64_t axon_linear_ce_grad_workspace_bytes(int64_t m, int64_t k, int64_t v,
+                                                     const axon_tune_t* tune);
+AXON_API int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const float* lse,
+                                 const float* loss_rows, const float* dloss, void* dh, void* dw,
+                                 int64_t m, int64_t k, int64_t v, int64_t ld_h, int64_t ld_w,
+                                 int64_t ld_dh, int64_t ld_dw, int32_t dtype, int32_t dw_dtype,
+                                 int32_t target_bits, int64_t ignore_index, int32_t reduction,
+                                 void* workspace, int64_t workspace_bytes, const axon_tune_t* tune,
+                                 void* stream);
+
+/* Synchronise `stream` and report whether one of the two calls since the last
+ * query gave up on a bounded pipeline wait (AXON_E_TIMEOUT; then cleared). */
+AXON_API int axon_linear_ce_status(void* stream);
+
 /* ---- tensor-parallel SwiGLU over NVLink peer memory ----------------------- */
 
 /* The reference's TP MLP resolves the down projection's Partial(+) output with

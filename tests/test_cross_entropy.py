@@ -1,0 +1,495 @@
+"""The output head's softmax cross entropy and its gradient against float64.
+
+Tolerances, from the arithmetic (u = half a step of the operand type, U = 2^-24):
+* a logit is a sum of k products that are exact in fp32; the tensor core adds
+  them 16 at a time, each addition off by at most 2^-23 of the magnitudes that
+  are summed (it may truncate), so |ds| <= (k/16 + 4) 2^-23 A, A the largest
+  sum over k of |h w|;
+* an exponential is off by 2^-22 of itself and by its argument's rounding,
+  2^-24 of at most 2^7: together E = 2^-16 covers it;
+* log-sum-exp: |ds| + E and one rounding; the loss of a row depends on logit
+  differences weighted with 1 - p_t <= min(1, loss), so min(1, loss) (2 |ds| + E) and a
+  rounding (losses are summed in float64);
+* an entry of d is off by r = 2 |ds| + 2 E + u of itself (f16: and by 2^-39 of
+  the largest |g|, half a step of subnormals at the scale it is held in); its
+  contraction by r and by (terms/16 + 4) 2^-23 of the sum of magnitudes; the
+  output by u of itself (f16: and half a step of subnormals, 2^-25);
+* what lies below the types' range: an fp32 loss under 2^-149 has no digits
+  (2^-150 beside the rounding), exponentials under 2^-126 are flushed (2^-126 of
+  the largest |g| beside an entry of d), and a bf16 output has steps of 2^-133
+  (2^-134 beside its rounding).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from enzyme_b200 import _native as N
+from enzyme_b200 import ops
+
+U32 = 2.0 ** -24
+E = 2.0 ** -16
+IGNORE = -100
+
+
+# ---- refusals (no GPU) --------------------------------------------------------------
+
+FAKE = ctypes.c_void_p(0x10000)  # never dereferenced: every call below is refused on the host
+BIG = 1 << 40
+
+
+def _fwd(**kw):
+    a = dict(h=FAKE, w=FAKE, t=FAKE, lse=FAKE, rows=FAKE, loss=FAKE, m=4, k=64, v=100, ldh=64, ldw=64, dt=N.AXON_BF16,
+             bits=64, red=N.AXON_REDUCE_MEAN, ws=FAKE, wsb=BIG, tune=None)
+    a.update(kw)
+    return N.lib().axon_linear_ce(a["h"], a["w"], a["t"], a["lse"], a["rows"], a["loss"], a["m"], a["k"], a["v"],
+                                  a["ldh"], a["ldw"], a["dt"], a["bits"], IGNORE, a["red"], a["ws"], a["wsb"],
+                                  a["tune"], None)
+
+
+def _bwd(**kw):
+    a = dict(h=FAKE, w=FAKE, t=FAKE, lse=FAKE, rows=FAKE, dloss=FAKE, dh=FAKE, dw=FAKE, m=4, k=64, v=100, ldh=64,
+             ldw=64, lddh=64, lddw=64, dt=N.AXON_BF16, dwt=N.AXON_BF16, bits=64, red=N.AXON_REDUCE_MEAN, ws=FAKE,
+             wsb=BIG, tune=None)
+    a.update(kw)
+    return N.lib().axon_linear_ce_grad(a["h"], a["w"], a["t"], a["lse"], a["rows"], a["dloss"], a["dh"], a["dw"],
+                                       a["m"], a["k"], a["v"], a["ldh"], a["ldw"], a["lddh"], a["lddw"], a["dt"],
+                                       a["dwt"], a["bits"], IGNORE, a["red"], a["ws"], a["wsb"], a["tune"], None)
+
+
+SHARED = [
+    (dict(m=-1), N.AXON_E_SHAPE), (dict(k=0), N.AXON_E_SHAPE), (dict(v=0), N.AXON_E_SHAPE),
+    (dict(k=60, ldh=64), N.AXON_E_SHAPE), (dict(m=1 << 31), N.AXON_E_SHAPE), (dict(v=1 << 31), N.AXON_E_SHAPE),
+    (dict(dt=N.AXON_F32), N.AXON_E_UNSUPPORTED), (dict(bits=16), N.AXON_E_UNSUPPORTED), (dict(red=3), N.AXON_E_ARG),
+    (dict(h=None), N.AXON_E_ARG), (dict(w=None), N.AXON_E_ARG), (dict(t=None), N.AXON_E_ARG),
+    (dict(lse=None), N.AXON_E_ARG), (dict(rows=None), N.AXON_E_ARG),
+    (dict(ldh=56), N.AXON_E_SHAPE), (dict(ldw=56), N.AXON_E_SHAPE), (dict(ldh=68), N.AXON_E_ALIGN),
+    (dict(ldw=68), N.AXON_E_ALIGN), (dict(h=ctypes.c_void_p(0x10008)), N.AXON_E_ALIGN),
+    (dict(w=ctypes.c_void_p(0x10002)), N.AXON_E_ALIGN), (dict(t=ctypes.c_void_p(0x10004)), N.AXON_E_ALIGN),
+    (dict(ws=None), N.AXON_E_ARG), (dict(wsb=16), N.AXON_E_ARG), (dict(ws=ctypes.c_void_p(0x10008)), N.AXON_E_ALIGN),
+    (dict(tune=ctypes.byref(N.Tune(variant=1))), N.AXON_E_ARG),
+    (dict(tune=ctypes.byref(N.Tune(max_ctas=-1))), N.AXON_E_ARG),
+]
+
+
+@pytest.mark.parametrize("i", range(len(SHARED)))
+def test_bad_arguments_are_refused(i):
+    kw, code = SHARED[i]
+    assert _fwd(**kw) == code, N.last_error()
+    assert _bwd(**kw) == code, N.last_error()
+    assert N.last_error().startswith("axon_linear_ce_grad")
+
+
+def test_more_refusals():
+    assert _fwd(loss=None) == N.AXON_E_ARG
+    for kw, code in ((dict(dloss=None), N.AXON_E_ARG), (dict(dh=None, dw=None), N.AXON_E_ARG),
+                     (dict(dwt=N.AXON_F16), N.AXON_E_UNSUPPORTED), (dict(lddh=56), N.AXON_E_SHAPE),
+                     (dict(lddw=68), N.AXON_E_ALIGN), (dict(dh=ctypes.c_void_p(0x10008)), N.AXON_E_ALIGN),
+                     (dict(tune=ctypes.byref(N.Tune(split=100))), N.AXON_E_ARG),
+                     (dict(ws=ctypes.c_void_p(0x10080)), N.AXON_E_ALIGN)):
+        assert _bwd(**kw) == code, (kw, N.last_error())
+
+
+def test_workspaces():
+    """The loss needs 8 bytes per row and 256 words; the gradient holds d by
+    pieces of at most 512 MB, and an fp32 dh only where there are several."""
+    lib = N.lib()
+    assert lib.axon_linear_ce_workspace_bytes(4096, 4096, 128256) < 4096 * 501 * 8 + 4096 * 4 + 1024
+    assert lib.axon_linear_ce_workspace_bytes(4, 60, 100) == N.AXON_E_SHAPE
+    one = lib.axon_linear_ce_grad_workspace_bytes(256, 64, 1000, None)
+    assert one < 256 * 1024 * 2 + 256 * 64 * 2 + 256 * 20 + 2048
+    two = lib.axon_linear_ce_grad_workspace_bytes(256, 64, 1000, N.Tune.of({"split": 512}))
+    assert two == one - 256 * 512 * 2 + 256 * 64 * 4
+    big = lib.axon_linear_ce_grad_workspace_bytes(16384, 4096, 128256, None)
+    assert big < (512 << 20) + 16384 * 4096 * 6 + 16384 * 20 + 4096
+
+
+def test_host_tensors_are_refused():
+    h, w, t = torch.zeros(2, 8).bfloat16(), torch.zeros(5, 8).bfloat16(), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(N.AxonError) as e:
+        ops.linear_cross_entropy(h, w, t)
+    assert e.value.code == N.AXON_E_ARG and "CUDA" in e.value.message
+
+
+# ---- GPU ----------------------------------------------------------------------------
+
+
+def _inputs(dev, m, k, v, dtype, seed=0, ignored=0.0, pull=10.0, pad=0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    h = torch.randn(m, k + pad, device=dev, generator=g)
+    w = (torch.randn(v, k + pad, device=dev, generator=g) * (1.3 / math.sqrt(k))).to(dtype)
+    t = torch.randint(0, v, (m,), device=dev, generator=g)
+    wt = w[t][:, :k].float()
+    h[:, :k] += pull * torch.rand(m, 1, device=dev, generator=g) * wt / wt.norm(dim=1, keepdim=True).clamp(min=1e-6)
+    if ignored:
+        t = torch.where(torch.rand(m, device=dev, generator=g) < ignored, torch.full_like(t, IGNORE), t)
+    return h.to(dtype)[:, :k], w[:, :k], t
+
+
+class Ref:
+    """Float64 evaluation with the bounds of the module's comment."""
+
+    def __init__(self, h, w, t, g=None):
+        self.m, self.k = h.shape
+        self.v = w.shape[0]
+        self.dtype = h.dtype
+        h, w = h.double(), w.double()
+        s = h @ w.T
+        self.keep = t != IGNORE
+        at = t.clamp(min=0).long()
+        rows = torch.arange(self.m, device=h.device)
+        st = s[rows, at]
+        other = s.clone()
+        other[rows[self.keep], at[self.keep]] = -math.inf
+        rest = torch.logsumexp(other, dim=1)
+        zero = torch.zeros_like(rest)
+        self.loss = torch.where(self.keep, torch.logaddexp(rest - st, zero), zero)
+        self.lse = torch.where(self.keep, torch.logaddexp(rest, st), rest)
+        a = float((h.abs() @ w.abs().T).max()) if self.m else 0.0
+        self.ds = (self.k / 16 + 4) * 2.0 ** -23 * a
+        self.u = torch.finfo(self.dtype).eps / 2
+        if g is not None:
+            g = torch.where(self.keep, g.double(), zero)
+            d = torch.exp(s - self.lse[:, None])
+            d[rows[self.keep], at[self.keep]] = torch.expm1(-self.loss)[self.keep]
+            d *= g[:, None]
+            r = 2 * self.ds + 2 * E + self.u
+            dd = d.abs() * r + float(g.abs().max()) * 2.0 ** -126 * self.keep[:, None]
+            floor = 2.0 ** -134
+            if self.dtype == torch.float16:
+                dd = dd + float(g.abs().max()) * 2.0 ** -39 * self.keep[:, None]
+                floor = 2.0 ** -25
+            self.dh, self.dw = d @ w, d.T @ h
+            self.dh_tol = (dd + (self.v / 16 + 4) * 2.0 ** -23 * d.abs()) @ w.abs() + self.u * self.dh.abs() + floor
+            # several pieces add one fp32 rounding of the sum each
+            self.dh_tol += 64 * U32 * (d.abs() @ w.abs())
+            self.dw_tol = (dd + (self.m / 16 + 4) * 2.0 ** -23 * d.abs()).T @ h.abs() + self.u * self.dw.abs() + floor
+
+    def check_loss(self, stats):
+        lse_err = (stats[0].double() - self.lse).abs()
+        assert bool((lse_err <= self.ds + E + U32 * self.lse.abs()).all()), float(lse_err.max())
+        err = (stats[1].double() - self.loss).abs()
+        tol = self.loss.clamp(max=1.0) * (2 * self.ds + E) + U32 * self.loss + 2.0 ** -150
+        assert bool((err <= tol).all()), float((err - tol).max())
+
+    def check_grads(self, dh, dw):
+        if dh is not None:
+            over = (dh.double() - self.dh).abs() - self.dh_tol
+            assert bool((over <= 0).all()), float(over.max())
+        if dw is not None:
+            over = (dw.double() - self.dw).abs() - self.dw_tol
+            assert bool((over <= 0).all()), float(over.max())
+
+
+def _both(h, w, t, dloss, reduction, **kw):
+    loss, stats = ops.linear_cross_entropy(h, w, t, reduction=reduction)
+    dh, dw = ops.linear_cross_entropy_grad(h, w, t, stats, dloss, reduction=reduction, **kw)
+    ops.linear_cross_entropy_status()
+    return loss, stats, dh, dw
+
+
+def _row_g(dloss, t, reduction):
+    keep = t != IGNORE
+    if reduction == "mean":
+        dloss = dloss / keep.sum()
+    return dloss.expand(t.shape)
+
+
+SHAPES = [
+    (1, 8, 1), (1, 64, 2), (2, 72, 255), (7, 64, 256), (1, 512, 5003), (37, 136, 257), (128, 64, 1000),
+    (129, 200, 513), (255, 256, 511), (256, 264, 768), (257, 512, 2049), (513, 128, 4099),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_loss(shape, dtype, cuda_device):
+    m, k, v = shape
+    h, w, t = _inputs(cuda_device, m, k, v, dtype, seed=m + v, ignored=0.2)
+    ref = Ref(h, w, t)
+    for reduction in ("none", "sum", "mean"):
+        loss, stats = ops.linear_cross_entropy(h, w, t, reduction=reduction)
+        ops.linear_cross_entropy_status()
+        ref.check_loss(stats)
+        rows = stats[1].double()
+        if reduction == "none":
+            assert torch.equal(loss, stats[1])
+        elif reduction == "sum":
+            assert torch.equal(loss, rows.sum().float()) or abs(float(loss - rows.sum())) <= 2 * U32 * float(rows.sum())
+        elif bool(ref.keep.any()):
+            mean = float(rows.sum() / ref.keep.sum())
+            assert abs(float(loss) - mean) <= 2 * U32 * mean
+        else:
+            assert loss.isnan()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gradients(shape, dtype, reduction, cuda_device):
+    m, k, v = shape
+    h, w, t = _inputs(cuda_device, m, k, v, dtype, seed=m + v, ignored=0.0 if m < 3 else 0.3)
+    if reduction == "none":
+        dloss = torch.randn(m, device=cuda_device, generator=torch.Generator(device=cuda_device).manual_seed(1))
+    else:
+        dloss = torch.full((1,), 16.0, device=cuda_device)
+    loss, stats, dh, dw = _both(h, w, t, dloss, reduction)
+    ref = Ref(h, w, t, _row_g(dloss, t, reduction))
+    ref.check_loss(stats)
+    ref.check_grads(dh, dw)
+    assert not bool(dh[~ref.keep].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [256, 512, 1024])
+@pytest.mark.parametrize("shape", [(5, 64, 1000), (300, 264, 2049), (513, 512, 1281)])
+def test_pieces_of_the_vocabulary(shape, split, cuda_device):
+    m, k, v = shape
+    for dtype in (torch.bfloat16, torch.float16):
+        h, w, t = _inputs(cuda_device, m, k, v, dtype, seed=split, ignored=0.1)
+        dloss = torch.ones(1, device=cuda_device)
+        _, _, dh, dw = _both(h, w, t, dloss, "sum", tune={"split": split})
+        Ref(h, w, t, _row_g(dloss, t, "sum")).check_grads(dh, dw)
+
+
+@pytest.mark.gpu
+def test_strides_types_and_parts(cuda_device):
+    """Padded leading dimensions in and out (what lies beside the outputs is
+    left alone), 32-bit targets, dw in fp32, one gradient without the other."""
+    m, k, v = 130, 72, 300
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=4, ignored=0.1, pad=24)
+    assert h.stride(0) == k + 24 and w.stride(0) == k + 24
+    dloss = torch.ones(1, device=cuda_device)
+    ref = Ref(h, w, t, _row_g(dloss, t, "mean"))
+    dh_room = torch.full((m, k + 8), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    dw_room = torch.full((v, k + 16), 7.0, device=cuda_device)
+    _, stats, dh, dw = _both(h, w, t.int(), dloss, "mean", out=(dh_room[:, :k], dw_room[:, :k]))
+    ref.check_grads(dh, dw)
+    assert bool((dh_room[:, k:] == 7).all()) and bool((dw_room[:, k:] == 7).all())
+    _, _, dh2, none = _both(h, w, t, dloss, "mean", need=(True, False))
+    assert none is None and torch.equal(dh2, dh)
+    _, _, none, dw2 = _both(h, w, t, dloss, "mean", need=(False, True), dw_dtype=torch.float32)
+    assert none is None and torch.equal(dw2, dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_against_differences(dtype, cuda_device):
+    """Central differences of the forward loss along random directions that the
+    operand type represents exactly (single entries moved by a power of two)."""
+    m, k, v = 6, 64, 40
+    h, w, t = _inputs(cuda_device, m, k, v, dtype, seed=11, pull=3.0)
+    dloss = torch.ones(1, device=cuda_device)
+    _, _, dh, dw = _both(h, w, t, dloss, "sum")
+    ref = Ref(h, w, t, _row_g(dloss, t, "sum"))
+
+    def loss_at(h, w):
+        return float(ops.linear_cross_entropy(h, w, t, reduction="none")[0].double().sum())
+
+    step = 2.0 ** -5
+    for x, grad, tol in ((h, dh, ref.dh_tol), (w, dw, ref.dw_tol)):
+        for i, j in ((0, 0), (3, 17), (5, 63), (1, 40)):
+            up, down = x.clone(), x.clone()
+            up[i, j] += step
+            down[i, j] -= step
+            span = float(up[i, j].double() - down[i, j].double())
+            args = ((up, w), (down, w)) if x is h else ((h, up), (h, down))
+            diff = (loss_at(*args[0]) - loss_at(*args[1])) / span
+            # third derivative of a log-sum-exp along a coordinate: at most the other operand's entry cubed
+            other = float((w if x is h else h).double().abs().max())
+            curve = (m if x is w else 1) * other ** 3 * span ** 2 / 8
+            centre = abs(float((up[i, j].double() + down[i, j].double()) / 2 - x[i, j].double())) * other ** 2 * m
+            noise = 2 * m * (2 * ref.ds + E + 8 * U32) / span
+            assert abs(diff - float(grad[i, j])) <= curve + centre + noise + float(tol[i, j])
+
+
+@pytest.mark.gpu
+def test_rows_that_do_not_count(cuda_device):
+    """Ignored rows may hold NaN and infinities; no row counted gives zero
+    gradients (mean: a NaN loss); no rows at all."""
+    m, k, v = 300, 64, 500
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=2, ignored=0.4)
+    keep = t != IGNORE
+    dloss = torch.ones(1, device=cuda_device)
+    loss, _, dh, dw = _both(h, w, t, dloss, "mean")
+    bad = h.clone()
+    idx = (~keep).nonzero().flatten()
+    bad[idx[0]] = float("nan")
+    bad[idx[1]] = float("inf")
+    bad[idx[2]] = torch.finfo(torch.bfloat16).min
+    loss2, stats2, dh2, dw2 = _both(bad, w, t, dloss, "mean")
+    assert torch.equal(loss, loss2) and torch.equal(dh, dh2) and torch.equal(dw, dw2)
+    assert bool(stats2[0][idx[0]].isnan()) and bool((stats2[1][~keep] == 0).all())
+    none = torch.full_like(t, IGNORE)
+    loss, stats, dh, dw = _both(bad, w, none, dloss, "mean")
+    assert loss.isnan() and not bool(stats[1].any()) and not bool(dh.any()) and not bool(dw.any())
+    loss, _, dh, dw = _both(bad, w, none, dloss, "sum")
+    assert float(loss) == 0.0 and not bool(dh.any()) and not bool(dw.any())
+    for reduction, want in (("sum", 0.0), ("mean", float("nan")), ("none", None)):
+        dl = torch.ones(0 if reduction == "none" else 1, device=cuda_device)
+        dw_out = torch.full((v, k), 3.0, dtype=torch.bfloat16, device=cuda_device)
+        loss, stats = ops.linear_cross_entropy(h[:0], w, t[:0], reduction=reduction)
+        dh, dw = ops.linear_cross_entropy_grad(h[:0], w, t[:0], stats, dl, reduction=reduction,
+                                               out=(torch.empty_like(h[:0]), dw_out))
+        assert stats.shape == (2, 0) and dh.shape == (0, k) and not bool(dw.any())
+        assert want is None or float(loss) == want or (math.isnan(want) and loss.isnan())
+
+
+@pytest.mark.gpu
+def test_targets_outside_the_vocabulary(cuda_device):
+    m, k, v = 40, 64, 100
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=6)
+    for bad in (-1, v, 2 ** 31, -(2 ** 40)):
+        t2 = t.clone()
+        t2[5] = bad
+        loss, stats = ops.linear_cross_entropy(h, w, t2, reduction="none")
+        good = torch.ones(m, dtype=torch.bool, device=cuda_device)
+        good[5] = False
+        assert loss[5].isnan() and not bool(loss[good].isnan().any()) and not bool(stats[0].isnan().any())
+        dh, dw = ops.linear_cross_entropy_grad(h, w, t2, stats, torch.ones(m, device=cuda_device), reduction="none")
+        assert bool(dh[5].isnan().all()) and not bool(dh[good].isnan().any()) and bool(dw.isnan().all())
+    # another ignored index, inside the vocabulary's range
+    t2 = t.clone()
+    t2[::3] = 0
+    loss, stats = ops.linear_cross_entropy(h, w, t2, ignore_index=0, reduction="none")
+    assert bool((loss[t2 == 0] == 0).all()) and bool((loss[t2 != 0] > 0).all())
+
+
+@pytest.mark.gpu
+def test_extreme_logits(cuda_device):
+    """Logits of several hundreds (no overflow), an almost certain target (the
+    loss keeps its digits), equal logits, and infinities."""
+    k, v = 64, 1000
+    for dtype in (torch.bfloat16, torch.float16):
+        h, w, t = _inputs(cuda_device, 20, k, v, dtype, seed=8)
+        big = h * 64
+        dloss = torch.ones(1, device=cuda_device)
+        _, stats, dh, dw = _both(big, w, t, dloss, "sum")
+        ref = Ref(big, w, t, _row_g(dloss, t, "sum"))
+        ref.check_loss(stats)
+        ref.check_grads(dh, dw)
+        # the target's logit is far above: losses down to 1e-12
+        w2 = w * 0.1
+        w2[3] = 1.0
+        h2 = torch.full((4, k), 0.25, device=cuda_device).to(dtype) * torch.arange(1, 5, device=cuda_device).to(
+            dtype)[:, None] * 0.5
+        t2 = torch.full((4,), 3, device=cuda_device)
+        _, stats, dh, dw = _both(h2, w2, t2, dloss, "sum")
+        ref = Ref(h2, w2, t2, _row_g(dloss, t2, "sum"))
+        assert float(ref.loss.min()) < 1e-9
+        ref.check_loss(stats)
+        ref.check_grads(dh, dw)
+        loss, stats = ops.linear_cross_entropy(torch.zeros_like(h), w, t, reduction="none")
+        assert bool(((loss - math.log(v)).abs() <= E).all())
+    h = torch.ones(3, k, device=cuda_device).bfloat16()
+    w = torch.zeros(v, k, device=cuda_device).bfloat16()
+    w[7] = float("-inf")
+    loss, stats = ops.linear_cross_entropy(h, w, torch.tensor([0, 7, IGNORE], device=cuda_device), reduction="none")
+    assert abs(float(loss[0]) - math.log(v - 1)) <= E and float(loss[1]) == float("inf")
+    assert bool(((stats[0] - math.log(v - 1)).abs() <= E).all())
+    w[7] = float("inf")
+    loss, _ = ops.linear_cross_entropy(h, w, torch.tensor([0, 7, IGNORE], device=cuda_device), reduction="none")
+    assert bool(loss[:2].isnan().all()) and float(loss[2]) == 0.0
+
+
+@pytest.mark.gpu
+def test_fp16_scales(cuda_device):
+    """fp16 gradients hold at loss scales far from one, and rows of very
+    different weight in one call."""
+    h, w, t = _inputs(cuda_device, 70, 64, 3000, torch.float16, seed=12, ignored=0.2)
+    for s in (2.0 ** -10, 1.0, 2.0 ** 15):
+        dloss = torch.full((1,), s, device=cuda_device)
+        _, _, dh, dw = _both(h, w, t, dloss, "mean")
+        Ref(h, w, t, _row_g(dloss, t, "mean")).check_grads(dh, dw)
+    dloss = 10.0 ** torch.linspace(-3, 2, 70, device=cuda_device)
+    _, _, dh, dw = _both(h, w, t, dloss, "none")
+    Ref(h, w, t, dloss).check_grads(dh, dw)
+    dloss[:] = 0
+    _, _, dh, dw = _both(h, w, t, dloss, "none")
+    assert not bool(dh.any()) and not bool(dw.any())
+
+
+@pytest.mark.gpu
+def test_wider_head(cuda_device):
+    """Several tiles in every direction, more tiles than pairs, default piece
+    and forced ones, bitwise repeatable."""
+    m, k, v = 1111, 1032, 20011
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=21, ignored=0.5)
+    dloss = torch.ones(1, device=cuda_device)
+    loss, stats, dh, dw = _both(h, w, t, dloss, "mean")
+    ref = Ref(h, w, t, _row_g(dloss, t, "mean"))
+    ref.check_loss(stats)
+    ref.check_grads(dh, dw)
+    again = _both(h, w, t, dloss, "mean")
+    for a, b in zip((loss, stats, dh, dw), again):
+        assert torch.equal(a, b)
+    _, _, dh, dw = _both(h, w, t, dloss, "mean", tune={"split": 4096, "max_ctas": 40})
+    ref.check_grads(dh, dw)
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graph(cuda_device):
+    """On a side stream, and captured twice with replays on new values."""
+    m, k, v = 200, 128, 1500
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=31, ignored=0.2)
+    dloss = torch.ones(1, device=cuda_device)
+    s = torch.cuda.Stream(cuda_device)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = _both(h, w, t, dloss, "mean")
+    torch.cuda.current_stream().wait_stream(s)
+    here = _both(h, w, t, dloss, "mean")
+    for a, b in zip(side, here):
+        assert torch.equal(a, b)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            loss, stats = ops.linear_cross_entropy(h, w, t)
+            grads = ops.linear_cross_entropy_grad(h, w, t, stats, dloss)
+        graphs.append((g, loss, stats, *grads))
+    for i in range(4):
+        hn, _, tn = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=40 + i, ignored=0.1 * i)
+        h.copy_(hn)
+        t.copy_(tn)
+        g, *got = graphs[i % 2]
+        g.replay()
+        want = _both(h, w, t, dloss, "mean")
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_wrapper_refusals(cuda_device):
+    h, w, t = _inputs(cuda_device, 4, 64, 50, torch.bfloat16)
+    _, stats = ops.linear_cross_entropy(h, w, t)
+    one = torch.ones(1, device=cuda_device)
+
+    def code(f):
+        with pytest.raises(N.AxonError) as e:
+            f()
+        return e.value.code
+
+    assert code(lambda: ops.linear_cross_entropy(h, w[:, :32], t)) == N.AXON_E_SHAPE
+    assert code(lambda: ops.linear_cross_entropy(h, w.half(), t)) == N.AXON_E_UNSUPPORTED
+    assert code(lambda: ops.linear_cross_entropy(h.float(), w.float(), t)) == N.AXON_E_UNSUPPORTED
+    assert code(lambda: ops.linear_cross_entropy(h, w, t[:3])) == N.AXON_E_SHAPE
+    assert code(lambda: ops.linear_cross_entropy(h, w, t.float())) == N.AXON_E_UNSUPPORTED
+    assert code(lambda: ops.linear_cross_entropy(h, w, t, reduction="max")) == N.AXON_E_ARG
+    assert code(lambda: ops.linear_cross_entropy(h[:, 1:57], w[:, 1:57], t)) == N.AXON_E_ALIGN
+    assert code(lambda: ops.linear_cross_entropy(h.T, w, t)) == N.AXON_E_SHAPE
+    grad = ops.linear_cross_entropy_grad
+    assert code(lambda: grad(h, w, t, stats[:, :3], one)) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, torch.ones(4, device=cuda_device))) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one, reduction="none")) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one.double())) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one, need=(False, False))) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one, dw_dtype=torch.float16)) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one, tune={"split": 100})) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one, out=(h[:2], w))) == N.AXON_E_ARG
