@@ -53,11 +53,21 @@ constexpr int A_BYTES = BM * BK * 2;
 constexpr int B_BYTES = BH * BK * 2;
 constexpr int STAGE = A_BYTES + B_BYTES;
 constexpr int CHUNK = 64 * BK * 2;   // one 64 x 64 block of an MN-major operand
-constexpr int kStages = 7;           // 7 x 32 KB of the 227 KB
+constexpr int kStaging = 32 * 128;   // 32 rows x 128 bytes for each warp that writes tiles
 constexpr uint32_t TMEM_COLS = 2 * BN;
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode { kLse = 0, kDlogits = 1, kGrads = 2 };
+
+// Epilogue warps, and the 32 KB stages that fit the 227 KB. Two warps share a
+// TMEM lane quarter, half the columns each, where a tile is written: with few
+// k-blocks a tile the epilogue is the longest part. kLse has one per quarter, so
+// that a row's pair comes from one thread.
+constexpr int epi_warps(int mode) { return mode == kLse ? 4 : 8; }
+constexpr int stages_of(int mode) { return mode == kLse ? 7 : 6; }
+constexpr int pair_threads(int mode) { return 64 + 32 * epi_warps(mode); }
+constexpr int staging_of(int mode) { return mode == kLse ? 0 : epi_warps(mode) * kStaging; }
+constexpr int smem_of(int mode) { return stages_of(mode) * STAGE + staging_of(mode) + 1024 + 256; }
 
 // What ce_grad_rows hands to the kernels after it.
 struct RowHeader {
@@ -68,28 +78,33 @@ struct RowHeader {
 struct CeParams {
   CUtensorMap a, b;     // kLse, kDlogits: h, w.   kGrads, dh tiles: d, w's piece
   CUtensorMap a2, b2;   // kGrads, dw tiles: d transposed, h
+  CUtensorMap c;        // what the epilogue writes by TMA: kDlogits d, kGrads dw
   int m, v, k;          // rows (at most), words of this piece, hidden size
   const RowHeader* header;  // NULL: all m rows
   // kLse
   const void* targets;
   int target64;
   int64_t ignore_index;
-  float2* part;         // [m][word tiles]
+  float2* part;         // [m][parts]
+  int parts;            // word tiles (ce_pair) or CTAs (ce_narrow)
+  unsigned* done;       // counts ce_stats' CTAs; set to 0 here
   // kDlogits: per counted row
   const int* row_target;
   const float* row_lse;
   const float* row_g;
   const float* row_dt;
   int v0;               // first word of the piece
-  void* d;              // [rows rounded up to 256][ld_d]
+  void* d;              // [m][ld_d]
   int64_t ld_d;
   // kGrads
   const int* row_index; // counted row -> row of dh
   void* dh;
   void* dw;
   int64_t ld_dh, ld_dw;
-  float* acc;           // fp32 [rows rounded up][k] between pieces
+  float* acc;           // fp32 [splits][m][k]: dh between pieces, and its splits
   int first, last;      // this piece is the vocabulary's first / last
+  int splits;           // parts that dh's contraction over the piece is cut into
+  int word_tile;        // ce_narrow: words a tile
   int band;             // row tiles of s visited together
 };
 
@@ -113,80 +128,109 @@ __device__ __forceinline__ float exp_from(float x, float ref) { return ex2((x - 
 
 struct Tile {
   bool dw;          // kGrads: a tile of dw (else of dh)
-  int tm, tn, kb;   // row tile, column tile, k-blocks
+  int tm, tn;       // row tile, column tile
+  int k0, kb;       // first k-block, k-blocks
+  int split;        // kGrads, dh: which part of the contraction
 };
 
-struct Walk {
-  int pair, pairs, rows;
-};
+// What a tile costs beside its k-blocks, in k-blocks: filling the pipeline and
+// writing 128 KB.
+constexpr int kTileCost = 4;
 
-// The `i`-th tile of this pair; false past the last one.
+// Up to this many k-blocks a dw tile takes longer to write than to compute.
+constexpr int kFewRows = 8;
+
+// A pair's way through the tiles, worked out once.
 //
 // kLse, kDlogits: bands of `band` row tiles (so that a band of h stays in L2),
 // each band word tile by word tile.
 //
-// kGrads: dh tiles (a contraction over the whole piece) first, dealt in turn;
-// the pairs that got one fewer start their dw tiles earlier, by as many as fit
-// in one dh tile's time, and the rest of the dw tiles is dealt in turn. Row
-// tiles run fastest for dh and column tiles for dw, so that the pairs share
-// the words, then d, in L2.
+// kGrads: the dh tiles (a contraction over the whole piece, or one part of it)
+// are dealt in turn; the pairs that got one fewer take as many dw tiles as fit in
+// one dh tile's time, and the rest of the dw tiles is dealt in turn. Row tiles run
+// fastest for dh and column tiles for dw, so that the pairs share the words,
+// and d, in L2. With few rows, even pairs begin with dh and odd ones with dw: dh is
+// then bound by reading w and dw by writing, and memory that only writes moves
+// 3.9 TB/s here, against 6.6 both ways (gradients of 64 x 2048 x 32000: 120 us,
+// all pairs beginning with dh 127; with 4096 rows it costs 4%).
 template <int MODE>
-__device__ __forceinline__ bool tile_at(const CeParams& p, const Walk& w, int i, Tile& t) {
-  const int row_tiles = (w.rows + 2 * BM - 1) / (2 * BM);
-  if constexpr (MODE != kGrads) {
-    const int word_tiles = (p.v + BN - 1) / BN;
-    const int64_t at = static_cast<int64_t>(i) * w.pairs + w.pair;
-    if (at >= static_cast<int64_t>(row_tiles) * word_tiles) return false;
-    const int64_t per_band = static_cast<int64_t>(p.band) * word_tiles;
-    const int band = static_cast<int>(at / per_band);
-    const int64_t within = at - band * per_band;
-    const int rows = row_tiles - band * p.band < p.band ? row_tiles - band * p.band : p.band;
-    t.dw = false;
-    t.tm = band * p.band + static_cast<int>(within % rows);
-    t.tn = static_cast<int>(within / rows);
-    t.kb = (p.k + BK - 1) / BK;
-    return true;
-  } else {
-    const int col_tiles = (p.k + BN - 1) / BN;
-    const int word_tiles = (p.v + 2 * BM - 1) / (2 * BM);
-    const int n_dh = p.dh ? row_tiles * col_tiles : 0;
-    const int n_dw = p.dw ? word_tiles * col_tiles : 0;
-    const int kb_dh = (p.v + BK - 1) / BK, kb_dw = (w.rows + BK - 1) / BK;
-    const int odd = n_dh % w.pairs;  // pairs below this one have a dh tile more
-    const int mine = n_dh / w.pairs + (w.pair < odd ? 1 : 0);
-    int at;
-    if (i < mine) {
-      at = i * w.pairs + w.pair;
-      t.dw = false;
-      t.tm = at % row_tiles;
-      t.tn = at / row_tiles;
-      t.kb = kb_dh;
-      return true;
+struct Walk {
+  int pair, pairs, rows;
+  int row_tiles, word_tiles, col_tiles;
+  int kb_all, kb_dh, kb_dw;
+  int mine, mine_dw, early, odd, behind;
+
+  __device__ __forceinline__ Walk(const CeParams& p, int rows_) {
+    pair = blockIdx.x >> 1;
+    pairs = gridDim.x >> 1;
+    rows = rows_;
+    row_tiles = (rows + 2 * BM - 1) / (2 * BM);
+    if constexpr (MODE != kGrads) {
+      word_tiles = (p.v + BN - 1) / BN;
+      kb_all = (p.k + BK - 1) / BK;
+    } else {
+      word_tiles = (p.v + 2 * BM - 1) / (2 * BM);
+      col_tiles = (p.k + BN - 1) / BN;
+      const int n_dh = p.dh ? row_tiles * col_tiles * p.splits : 0;
+      const int n_dw = p.dw ? word_tiles * col_tiles : 0;
+      kb_all = (p.v + BK - 1) / BK;
+      kb_dh = (kb_all + p.splits - 1) / p.splits;
+      kb_dw = (rows + BK - 1) / BK;
+      odd = n_dh % pairs;  // pairs below this one have a dh tile more
+      mine = n_dh / pairs + (pair < odd ? 1 : 0);
+      behind = odd ? pairs - odd : 0;                      // pairs with one dh tile fewer
+      early = (kb_dh + kTileCost) / (kb_dw + kTileCost);   // dw tiles they take meanwhile
+      if (behind == 0) early = 0;
+      else if (early > n_dw / behind) early = n_dw / behind;
+      const int rest = n_dw - behind * early;
+      mine_dw = (rest > pair ? (rest - pair + pairs - 1) / pairs : 0) + (pair >= odd ? early : 0);
     }
-    i -= mine;
-    const int behind = odd ? w.pairs - odd : 0;  // pairs with one dh tile fewer
-    int early = kb_dw > 0 ? kb_dh / kb_dw : 0;   // dw tiles they take meanwhile
-    if (behind && early > n_dw / behind) early = n_dw / behind;
-    if (behind && w.pair >= odd) {
-      if (i < early) {
-        at = i * behind + (w.pair - odd);
-        t.dw = true;
-        t.tm = at / col_tiles;
-        t.tn = at % col_tiles;
-        t.kb = kb_dw;
+  }
+
+  // The `i`-th tile of this pair; false past the last one.
+  __device__ __forceinline__ bool at(const CeParams& p, int i, Tile& t) const {
+    t.dw = false;
+    t.k0 = 0;
+    t.split = 0;
+    if constexpr (MODE != kGrads) {
+      int64_t at = static_cast<int64_t>(i) * pairs + pair;
+      if (at >= static_cast<int64_t>(row_tiles) * word_tiles) return false;
+      int first = 0, tiles = row_tiles;
+      if (row_tiles > p.band) {
+        const int64_t per_band = static_cast<int64_t>(p.band) * word_tiles;
+        first = static_cast<int>(at / per_band) * p.band;
+        at -= static_cast<int64_t>(first) * word_tiles;
+        tiles = row_tiles - first < p.band ? row_tiles - first : p.band;
+      }
+      t.tn = static_cast<int>(at / tiles);
+      t.tm = first + static_cast<int>(at - static_cast<int64_t>(t.tn) * tiles);
+      t.kb = kb_all;
+      return true;
+    } else {
+      if (i >= mine + mine_dw) return false;
+      if ((pair & 1) && kb_dw <= kFewRows) i = i < mine_dw ? mine + i : i - mine_dw;
+      if (i < mine) {
+        const int at = i * pairs + pair, rest = at / row_tiles;
+        t.tm = at - rest * row_tiles;
+        t.split = rest / col_tiles;
+        t.tn = rest - t.split * col_tiles;
+        t.k0 = t.split * kb_dh;
+        const int left = kb_all - t.k0;
+        t.kb = left < kb_dh ? (left > 0 ? left : 0) : kb_dh;
         return true;
       }
-      i -= early;
+      i -= mine;
+      t.dw = true;
+      t.kb = kb_dw;
+      int at;
+      if (pair >= odd && i < early) at = i * behind + (pair - odd);
+      else at = behind * early + (i - (pair >= odd ? early : 0)) * pairs + pair;
+      t.tm = at / col_tiles;
+      t.tn = at - t.tm * col_tiles;
+      return true;
     }
-    const int64_t rest = static_cast<int64_t>(behind) * early + static_cast<int64_t>(i) * w.pairs + w.pair;
-    if (rest >= n_dw) return false;
-    t.dw = true;
-    t.tm = static_cast<int>(rest / col_tiles);
-    t.tn = static_cast<int>(rest % col_tiles);
-    t.kb = kb_dw;
-    return true;
   }
-}
+};
 
 // One k-block of this CTA's half of the operands: 128 rows of A, 128 columns
 // of B, 32 KB. K-major operands come as 128 rows x 64 elements of k; MN-major
@@ -194,6 +238,7 @@ __device__ __forceinline__ bool tile_at(const CeParams& p, const Walk& w, int i,
 template <int MODE>
 __device__ __forceinline__ void load_stage(const CeParams& p, const Tile& t, int kb, int rank, uint8_t* sa,
                                            uint32_t full) {
+  kb += t.k0;
   uint8_t* sb = sa + A_BYTES;
   const int row0 = t.tm * 2 * BM + rank * BM;
   const int col0 = t.tn * BN + rank * BH;
@@ -266,58 +311,96 @@ __device__ __forceinline__ void lse_tile(const CeParams& p, const Tile& t, uint3
     sum = sum * exp_from(mx, ref) + ((s[0] + s[1]) + (s[2] + s[3]));
     mx = nm;
   }
-  if (row_ok) p.part[row * ((p.v + BN - 1) / BN) + t.tn] = make_float2(mx, sum);
+  if (row_ok) p.part[row * p.parts + t.tn] = make_float2(mx, sum);
 }
 
+// A thread holds a row of an accumulator tile, so its stores would touch 32 rows
+// an instruction. A warp's 32 rows x 128 bytes turn around in shared memory
+// instead, 16-byte pieces in the order of TMA's 128-byte swizzle, and leave by a
+// TMA store or in whole 128-byte row pieces.
+__device__ __forceinline__ uint4* staged(uint8_t* stg, int row, int piece) {
+  return reinterpret_cast<uint4*>(stg + row * 128 + ((piece ^ (row & 7)) << 4));
+}
+
+// This thread's row piece of 128 bytes into the staging memory.
 template <typename T>
-__device__ __forceinline__ void store32_full(T* dst, const float* v) {
+__device__ __forceinline__ void stage_row(uint8_t* stg, int lane, const float* v) {
+  constexpr int E = Vec<T>::E;
 #pragma unroll
-  for (int j = 0; j < 32; j += 8) {
+  for (int i = 0; i < 8; ++i) {
     Vec<T> pk;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) pk.e[e] = from_f<T>(v[j + e]);
-    st_vec(dst + j, pk);
+    for (int e = 0; e < E; ++e) pk.e[e] = from_f<T>(v[i * E + e]);
+    *staged(stg, lane, i) = pk.u;
   }
 }
 
-// kDlogits: d for this thread's row. Rows past the counted ones inside the
-// tile are written as zeros (the contraction over rows reads them), and so
-// are the words that pad ld_d.
+// The staged rows to (col, row) of the map, once all lanes have written theirs.
+__device__ __forceinline__ void store_staged(const CUtensorMap* map, uint8_t* stg, int lane, int col, int row) {
+  fence_async_smem();
+  __syncwarp();
+  if (lane == 0) tma_store_2d(map, stg, col, row);
+}
+
+// Before the staging memory is written again.
+__device__ __forceinline__ void staging_free(int lane) {
+  if (lane == 0) tma_store_wait_read();
+  __syncwarp();
+}
+
+// COLS accumulator columns from tensor memory.
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float* v) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < COLS; i += 32) tmem_ld32(taddr + i, v + i);
+  tmem_wait_ld();
+}
+
+// This warp is done with the accumulator (its values are in registers).
+__device__ __forceinline__ void release_tmem(uint32_t leader_tempty, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_cluster(leader_tempty, 1);
+}
+
+// Rows of d that the contraction over rows reads: the counted ones up to the
+// end of their k-block. Those past the counted ones are written as zeros; past
+// m TMA reads zeros by itself.
+__device__ __forceinline__ int rows_read(const CeParams& p, int rows) {
+  const int end = (rows + BK - 1) / BK * BK;
+  return end < p.m ? end : p.m;
+}
+
+// kDlogits: d for this thread's row in columns [c0, c0 + 128) of the tile. The
+// accumulator is released once its second half is in registers.
 template <typename T>
-__device__ __forceinline__ void dlogits_tile(const CeParams& p, const Tile& t, uint32_t tbase, int64_t row,
-                                             bool row_ok) {
+__device__ __forceinline__ void dlogits_tile(const CeParams& p, const Tile& t, uint32_t tbase, int c0, int64_t row0,
+                                             int lane, int rows, uint8_t* stg, uint32_t tempty) {
+  const int64_t row = row0 + lane;
+  const bool row_ok = row < rows, any = row0 < rows_read(p, rows);
   const float lse = row_ok ? p.row_lse[row] : 0.f;
   const float g = row_ok ? p.row_g[row] : 0.f;
+  const float dt = row_ok ? p.row_dt[row] : 0.f;
   const int target = row_ok ? p.row_target[row] - p.v0 : -1;
-  T* drow = static_cast<T*>(p.d) + row * p.ld_d;
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
-    const int col = t.tn * BN + c * 32;
-    if (col >= p.v) break;
-    float v[32];
-    __syncwarp();
-    tmem_ld32(tbase + c * 32, v);
-    tmem_wait_ld();
+  for (int c = 0; c < BN / 2; c += 64) {
+    const int col = t.tn * BN + c0 + c;
+    float v[64];
+    tmem_ld_cols<64>(tbase + c0 + c, v);
+    if (c + 64 == BN / 2) release_tmem(tempty, lane);
+    if (!any || col >= p.v) continue;  // the same for the whole warp
+    const int left = row_ok ? p.v - col : 0;  // words of this piece that count
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = row_ok && col + j < p.v ? exp_from(v[j], lse) * g : 0.f;
-    if (target >= col && target < col + 32) {
-      const float dt = p.row_dt[row];
+    for (int j = 0; j < 64; ++j) v[j] = j < left ? exp_from(v[j], lse) * g : 0.f;
+    if (target >= col && target < col + 64) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < 64; ++j)
         if (target == col + j) v[j] = dt;
     }
-    if (col + 32 <= p.ld_d) {
-      store32_full<T>(drow + col, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; j += 8)
-        if (col + j < p.ld_d) {
-          Vec<T> pk;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) pk.e[e] = from_f<T>(v[j + e]);
-          st_vec(drow + col + j, pk);
-        }
-    }
+    staging_free(lane);
+    stage_row<T>(stg, lane, v);
+    store_staged(&p.c, stg, lane, col, static_cast<int>(row0));
   }
 }
 
@@ -335,58 +418,85 @@ __device__ __forceinline__ void store8(TO* dst, const float* v) {
   }
 }
 
-// kGrads: this thread's row of a tile of dh or dw.
-template <typename T, typename TW>
-__device__ __forceinline__ void grad_tile(const CeParams& p, const Walk& w, const Tile& t, uint32_t tbase, int64_t row,
-                                          float unscale) {
-  const bool row_ok = t.dw ? row < p.v : row < w.rows;
-  const int64_t out_row = row_ok ? (t.dw ? p.v0 + row : (p.last ? p.row_index[row] : 0)) : 0;
+// kGrads, columns [c0, c0 + 128) of a tile of dw, rounded (row0 the warp's first
+// word within the piece). The accumulator is released once its last part is in
+// registers: with few rows a tile is one or two k-blocks, and the pair would
+// wait for its epilogue.
+template <typename TW>
+__device__ __forceinline__ void dw_tile(const CeParams& p, const Tile& t, uint32_t tbase, int c0, int64_t row0,
+                                        int lane, float unscale, uint8_t* stg, uint32_t tempty) {
+  constexpr int COLS = 128 / sizeof(TW);
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
-    const int col = t.tn * BN + c * 32;
+  for (int c = 0; c < BN / 2; c += COLS) {
+    const int col = t.tn * BN + c0 + c;
+    float v[COLS];
+    tmem_ld_cols<COLS>(tbase + c0 + c, v);
+    if (c + COLS == BN / 2) release_tmem(tempty, lane);
+    if (row0 >= p.v || col >= p.k) continue;  // the same for the whole warp
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) v[j] = t.kb ? v[j] * unscale : 0.f;  // no k-block: nothing was accumulated
+    staging_free(lane);
+    stage_row<TW>(stg, lane, v);
+    store_staged(&p.c, stg, lane, col, static_cast<int>(row0));
+  }
+}
+
+// kGrads, columns [c0, c0 + 128) of a tile of dh: added to the accumulator of its
+// split, or, where this piece and part are all there is left, rounded and
+// written to its row.
+template <typename T>
+__device__ __forceinline__ void dh_tile(const CeParams& p, const Tile& t, uint32_t tbase, int c0, int64_t row0,
+                                        int lane, int rows, float unscale, uint8_t* stg, uint32_t tempty) {
+  const bool direct = p.last && p.splits == 1;
+  float* acc = p.acc + (static_cast<int64_t>(t.split) * p.m + row0) * p.k;
+  staging_free(lane);
+#pragma unroll 1
+  for (int c = c0; c < c0 + BN / 2; c += 32) {
+    const int col = t.tn * BN + c;
     if (col >= p.k) break;
     float v[32];
-    __syncwarp();
-    tmem_ld32(tbase + c * 32, v);
-    tmem_wait_ld();
-    if (!row_ok) continue;
-    if (t.kb == 0) {  // no row counts: the accumulator was never written
+    tmem_ld_cols<32>(tbase + c, v);
+    if (t.kb == 0) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = 0.f;
     }
+    stage_row<float>(stg, lane, v);
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (col + j >= p.k) break;  // k is a multiple of 8
-      if (t.dw) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j + e] *= unscale;
-        store8<TW>(static_cast<TW*>(p.dw) + out_row * p.ld_dw + col + j, v + j);
-        continue;
-      }
-      float* acc = p.acc + row * p.k + col + j;
-      if (!p.first) {
-        const float4 a = *reinterpret_cast<const float4*>(acc), b = *reinterpret_cast<const float4*>(acc + 4);
-        v[j] += a.x; v[j + 1] += a.y; v[j + 2] += a.z; v[j + 3] += a.w;
-        v[j + 4] += b.x; v[j + 5] += b.y; v[j + 6] += b.z; v[j + 7] += b.w;
-      }
-      if (p.last) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j + e] *= unscale;
-        store8<T>(static_cast<T*>(p.dh) + out_row * p.ld_dh + col + j, v + j);
-      } else {
-        store8<float>(acc, v + j);
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3), piece = lane & 7;
+      if (row0 + r < rows && col + piece * 4 < p.k) {
+        float4 x = *reinterpret_cast<const float4*>(staged(stg, r, piece));
+        float4* at = reinterpret_cast<float4*>(acc + static_cast<int64_t>(r) * p.k + col + piece * 4);
+        if (!p.first) {
+          const float4 a = *at;
+          x.x += a.x; x.y += a.y; x.z += a.z; x.w += a.w;
+        }
+        if (direct) {
+          T* out = static_cast<T*>(p.dh) + p.row_index[row0 + r] * p.ld_dh + col + piece * 4;
+          union { T e[4]; uint2 u; } pk;
+          pk.e[0] = from_f<T>(x.x * unscale); pk.e[1] = from_f<T>(x.y * unscale);
+          pk.e[2] = from_f<T>(x.z * unscale); pk.e[3] = from_f<T>(x.w * unscale);
+          *reinterpret_cast<uint2*>(out) = pk.u;
+        } else {
+          *at = x;
+        }
       }
     }
+    __syncwarp();
   }
+  release_tmem(tempty, lane);
 }
 
 // ---- the CTA-pair kernel ---------------------------------------------------------------
 
 template <int MODE, typename T, typename TW>
-__global__ void __launch_bounds__(192, 1) ce_pair(const __grid_constant__ CeParams p) {
+__global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_constant__ CeParams p) {
+  constexpr int kStages = stages_of(MODE);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * STAGE);
+  uint8_t* staging = smem + kStages * STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + staging_of(MODE));
   uint64_t* empty = full + kStages;
   uint64_t* tfull = empty + kStages;
   uint64_t* tempty = tfull + 2;
@@ -407,7 +517,7 @@ __global__ void __launch_bounds__(192, 1) ce_pair(const __grid_constant__ CePara
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 8);  // one arrival per epilogue warp of each CTA
+      mbar_init(&tempty[b], 2 * epi_warps(MODE));  // one arrival per epilogue warp of each CTA
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -426,18 +536,19 @@ __global__ void __launch_bounds__(192, 1) ce_pair(const __grid_constant__ CePara
   cluster_barrier();  // both CTAs' barriers are initialised before either is addressed remotely
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
 
-  Walk w;
-  w.pair = blockIdx.x >> 1;
-  w.pairs = gridDim.x >> 1;
-  w.rows = p.header ? p.header->rows : p.m;
+  const Walk<MODE> w(p, p.header ? p.header->rows : p.m);
   Tile t;
+
+  if (MODE == kLse && blockIdx.x == 0 && threadIdx.x == 64) *p.done = 0;
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
     int stage = 0;
     uint32_t phase = 0;
-    for (int i = 0; tile_at<MODE>(p, w, i, t); ++i) {
+    for (int i = 0; w.at(p, i, t); ++i) {
       for (int kb = 0; kb < t.kb; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_ce_error)) goto producer_done;
         const uint32_t leader_full = mapa_u32(smem_u32(&full[stage]), 0);
@@ -455,7 +566,7 @@ __global__ void __launch_bounds__(192, 1) ce_pair(const __grid_constant__ CePara
     // ---------------- MMA issuer (leader only) ----------------
     int stage = 0;
     uint32_t phase = 0;
-    for (int i = 0; tile_at<MODE>(p, w, i, t); ++i) {
+    for (int i = 0; w.at(p, i, t); ++i) {
       const int buf = i & 1;
       if (!mbar_wait(&tempty[buf], ((i >> 1) & 1) ^ 1u, abort_flag, &g_ce_error)) break;
       tc_fence_after();
@@ -496,19 +607,25 @@ __global__ void __launch_bounds__(192, 1) ce_pair(const __grid_constant__ CePara
     // ---------------- epilogue (both CTAs, their own 128 rows) ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
     const float unscale = MODE == kGrads ? p.header->unscale : 1.f;
-    for (int i = 0; tile_at<MODE>(p, w, i, t); ++i) {
+    for (int i = 0; w.at(p, i, t); ++i) {
       const int buf = i & 1;
       if (!mbar_wait(&tfull[buf], (i >> 1) & 1, abort_flag, &g_ce_error)) break;
       tc_fence_after();
-      const int64_t row = static_cast<int64_t>(t.tm) * 2 * BM + rank * BM + q * 32 + lane;
+      const int64_t row0 = static_cast<int64_t>(t.tm) * 2 * BM + rank * BM + q * 32;  // of this warp's 32
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * BN);
-      if constexpr (MODE == kLse) lse_tile(p, t, tbase, row, row < w.rows);
-      else if constexpr (MODE == kDlogits) dlogits_tile<T>(p, t, tbase, row, row < w.rows);
-      else grad_tile<T, TW>(p, w, t, tbase, row, unscale);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&tempty[buf]), 0), 1);
+      const uint32_t leader_tempty = mapa_u32(smem_u32(&tempty[buf]), 0);
+      if constexpr (MODE == kLse) {
+        lse_tile(p, t, tbase, row0 + lane, row0 + lane < w.rows);
+        release_tmem(leader_tempty, lane);
+      } else {
+        uint8_t* stg = staging + (warp - 2) * kStaging;
+        const int c0 = warp < 6 ? 0 : BN / 2;  // this warp's half of the columns
+        if constexpr (MODE == kDlogits) dlogits_tile<T>(p, t, tbase, c0, row0, lane, w.rows, stg, leader_tempty);
+        else if (t.dw) dw_tile<TW>(p, t, tbase, c0, row0, lane, unscale, stg, leader_tempty);
+        else dh_tile<T>(p, t, tbase, c0, row0, lane, w.rows, unscale, stg, leader_tempty);
+      }
     }
+    if (MODE != kLse && lane == 0) tma_store_wait();
   }
 
   __syncthreads();
@@ -522,6 +639,256 @@ __global__ void __launch_bounds__(192, 1) ce_pair(const __grid_constant__ CePara
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS)
                  : "memory");
+  }
+}
+
+// ---- few rows: the words on the accumulator's lanes -----------------------------------------
+//
+// With at most 64 rows the products are bound by reading w once, and a tile of
+// 256 rows by 256 words would spend its shared memory and MMA time on rows that
+// are not there. Here the words are the MMA's M (128 a tile, one CTA) and the
+// rows its N (NT = 16, 32 or 64), so a k-block stages 16 KB of w beside 2-8 KB of
+// h, ten to twelve of them deep.
+//
+//   kLse      a thread owns a lane, so one word of each of its CTA's tiles, and
+//             keeps a running (max, sum) for every row in registers; the 128
+//             lanes are joined once, at the end, into one (max, sum) per row
+//             and CTA;
+//   kDlogits  a warp's 32 lanes are 32 neighbouring words of a row of d.
+constexpr int kNarrowRows = 64;
+constexpr int kNarrowMaxStages = 12;
+
+constexpr int narrow_stage(int nt) { return A_BYTES + nt * BK * 2; }
+constexpr int narrow_stages(int nt) {
+  const int fit = (232448 - 1024 - 1024) / narrow_stage(nt);
+  return fit < kNarrowMaxStages ? fit : kNarrowMaxStages;
+}
+
+// 32 lanes x 16 consecutive 32-bit TMEM columns.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Joins (max, sum) pairs.
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float mx = fmaxf(a.x, b.x);
+  const float ref = mx == __int_as_float(0xff800000) ? 0.f : mx;
+  return make_float2(mx, a.y * exp_from(a.x, ref) + b.y * exp_from(b.x, ref));
+}
+
+template <int MODE, typename T, int NT>
+__global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CeParams p) {
+  constexpr int S = narrow_stages(NT);
+  constexpr int SB = narrow_stage(NT);
+  constexpr uint32_t COLS = 2 * NT < 32 ? 32 : 2 * NT;
+  static_assert(S * SB >= 128 * NT * 8, "the lanes' pairs are joined in the stages' memory");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * SB);
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* issued = reinterpret_cast<int*>(tmem_slot + 2);
+  int* row_target = reinterpret_cast<int*>(tmem_slot + 4);  // [NT]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 4);  // one arrival per epilogue warp
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    *issued = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  pdl_wait();
+  pdl_trigger();
+  const int rows = p.header ? p.header->rows : p.m;
+  if (threadIdx.x < NT) {
+    const int r = threadIdx.x;
+    int t = -1;
+    if (r < rows) {
+      if constexpr (MODE == kLse) t = load_target(p.targets, p.target64, r, p.ignore_index, p.v);
+      else t = p.row_target[r] - p.v0;
+    }
+    row_target[r] = t;
+  }
+  if (MODE == kLse && blockIdx.x == 0 && threadIdx.x == 64) *p.done = 0;
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int tiles = rows > 0 ? (p.v + p.word_tile - 1) / p.word_tile : 0;
+  const uint32_t stage_bytes = static_cast<uint32_t>(p.word_tile * BK * 2 + NT * BK * 2);
+  const int kblocks = (p.k + BK - 1) / BK;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x)
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_ce_error)) goto producer_done;
+        mbar_expect_tx(&full[stage], stage_bytes);
+        uint8_t* sa = smem + stage * SB;
+        tma_load_2d(&p.a, &full[stage], sa, kb * BK, t * p.word_tile);
+        tma_load_2d(&p.b, &full[stage], sa + A_BYTES, kb * BK, 0);
+        *issued += 1;
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+  producer_done:;
+  } else if (warp == 1 && lane == 0) {
+    // ---------------- MMA issuer ----------------
+    constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t id = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(NT >> 3) << 17) |
+                            (static_cast<uint32_t>(BM >> 4) << 24);
+    int stage = 0;
+    uint32_t phase = 0;
+    int i = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+      const int buf = i & 1;
+      if (!mbar_wait(&tempty[buf], ((i >> 1) & 1) ^ 1u, abort_flag, &g_ce_error)) break;
+      tc_fence_after();
+      const uint32_t d = tmem_base + static_cast<uint32_t>(buf * NT);
+      bool ok = true;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, &g_ce_error)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + stage * SB);
+        const uint32_t sb = sa + A_BYTES;
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          tc_mma(d, sdesc(sa + k * 32, 16, 1024), sdesc(sb + k * 32, 16, 1024), id, (kb | k) != 0);
+        tc_commit(&empty[stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      tc_commit(&tfull[buf]);
+    }
+    // TMEM is released only after every MMA this thread issued has retired
+    tc_commit(drain);
+    volatile int never = 0;
+    mbar_wait(drain, 0, &never, &g_ce_error);
+  } else if (warp >= 2) {
+    // ---------------- epilogue ----------------
+    const float ninf = __int_as_float(0xff800000);
+    const int q = warp & 3;  // TMEM lane quarter this warp may access
+    float mx[MODE == kLse ? NT : 1], sm[MODE == kLse ? NT : 1];
+    if constexpr (MODE == kLse) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        mx[c] = ninf;
+        sm[c] = 0.f;
+      }
+    }
+    int i = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
+      const int buf = i & 1;
+      if (!mbar_wait(&tfull[buf], (i >> 1) & 1, abort_flag, &g_ce_error)) break;
+      tc_fence_after();
+      // lanes past the tile's words hold what the stage held before
+      const int word = q * 32 + lane < p.word_tile ? t * p.word_tile + q * 32 + lane : 0x7fffffff;
+      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * NT);
+      const int write = MODE == kDlogits ? rows_read(p, rows) : 0;
+#pragma unroll
+      for (int c0 = 0; c0 < NT; c0 += 16) {
+        if (c0 >= p.m) break;  // the same for the whole warp
+        float v[16];
+        __syncwarp();
+        tmem_ld16(tbase + c0, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int c = c0 + j;
+          if constexpr (MODE == kLse) {
+            const float x = word < p.v && row_target[c] != word ? v[j] : ninf;
+            const float nm = fmaxf(mx[c], x);
+            const float ref = nm == ninf ? 0.f : nm;
+            sm[c] = sm[c] * exp_from(mx[c], ref) + exp_from(x, ref);
+            mx[c] = nm;
+          } else {
+            if (c < write && word < p.ld_d) {
+              float x = 0.f;
+              if (c < rows && word < p.v)
+                x = row_target[c] == word ? p.row_dt[c] : exp_from(v[j], p.row_lse[c]) * p.row_g[c];
+              static_cast<T*>(p.d)[c * p.ld_d + word] = from_f<T>(x);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+    }
+    if constexpr (MODE == kLse) {
+      // every stage has been read (the last accumulator is done): its memory
+      // takes the lanes' pairs, a row of NT per lane
+      float2* lanes = reinterpret_cast<float2*>(smem);
+      const int l = q * 32 + lane;
+#pragma unroll
+      for (int c = 0; c < NT; ++c) lanes[l * NT + c] = make_float2(mx[c], sm[c]);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      constexpr int SEG = 128 / NT;  // threads that share a row
+      const int c = l % NT, seg = l / NT;
+      float2 s = make_float2(ninf, 0.f);
+#pragma unroll 16
+      for (int j = 0; j < NT; ++j) s.x = fmaxf(s.x, lanes[(seg * NT + j) * NT + c].x);
+      const float ref = s.x == ninf ? 0.f : s.x;
+#pragma unroll 16
+      for (int j = 0; j < NT; ++j) {
+        const float2 o = lanes[(seg * NT + j) * NT + c];
+        s.y += o.y * exp_from(o.x, ref);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      lanes[l] = s;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (l < rows) {
+        for (int j = 1; j < SEG; ++j) s = join(s, lanes[j * NT + l]);
+        p.part[static_cast<int64_t>(l) * p.parts + blockIdx.x] = s;
+      }
+    }
+  }
+
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && *issued > 0) {
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies issued may still be landing
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(COLS) : "memory");
   }
 }
 
@@ -541,61 +908,6 @@ __device__ __forceinline__ float warp_dot(const T* x, const T* y, int k, int lan
   return warp_sum(((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7])));
 }
 
-struct StatsArgs {
-  const void* h;
-  const void* w;
-  int64_t ld_h, ld_w;
-  const float2* part;
-  const void* targets;
-  int target64;
-  int64_t ignore_index;
-  int m, k, v, tiles;
-  float* lse;
-  float* loss;
-};
-
-// Joins a row's (max, sum) of every word tile with the target's logit, a warp
-// per row.
-template <typename T>
-__global__ void __launch_bounds__(128) ce_stats(StatsArgs a) {
-  const float ninf = __int_as_float(0xff800000);
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= a.m) return;
-  const int target = load_target(a.targets, a.target64, row, a.ignore_index, a.v);
-  float at = 0.f;
-  if (target >= 0)
-    at = warp_dot(static_cast<const T*>(a.h) + row * a.ld_h, static_cast<const T*>(a.w) + target * a.ld_w, a.k, lane);
-  const float2* pr = a.part + row * a.tiles;
-  float mx = ninf;
-  for (int i = lane; i < a.tiles; i += 32) mx = fmaxf(mx, pr[i].x);
-  mx = warp_max(mx);
-  const float ref = mx == ninf ? 0.f : mx;
-  float sum = 0.f;
-  for (int i = lane; i < a.tiles; i += 32) {
-    const float2 t = pr[i];
-    sum += t.y * exp_from(t.x, ref);
-  }
-  sum = warp_sum(sum);
-  if (lane) return;
-  // the log-sum-exp over the words other than the target, and the loss, in 64
-  // bits: a row each, and an almost certain target leaves a loss far below
-  // the logits' own rounding
-  const double rest = static_cast<double>(ref) + log(static_cast<double>(sum));
-  double lse = rest, loss = 0.0;
-  if (target >= 0) {
-    const double st = at;
-    const double x = rest - st;
-    loss = x > 0.0 ? x + log1p(exp(-x)) : log1p(exp(x));
-    lse = x > 0.0 ? rest + log1p(exp(-x)) : st + loss;
-    if (st > 3.5e38) loss = lse - st;  // an infinite logit: NaN, as lse - s_t says, not 0
-  } else if (target == -2) {
-    loss = __longlong_as_double(0x7ff8000000000000ll);
-  }
-  a.lse[row] = static_cast<float>(lse);
-  a.loss[row] = static_cast<float>(loss);
-}
-
 // CTA-wide sums in a fixed order, returned to every thread.
 template <typename V, int THREADS>
 __device__ __forceinline__ V cta_sum(V v) {
@@ -611,18 +923,88 @@ __device__ __forceinline__ V cta_sum(V v) {
   return s;
 }
 
-// Sum or mean of the rows' losses: one CTA, float64, fixed order.
-__global__ void __launch_bounds__(1024) ce_reduce(const float* __restrict__ loss_rows, const void* targets, int target64,
-                                                  int64_t ignore_index, int64_t v, int m, int mean, float* loss) {
+struct StatsArgs {
+  const void* h;
+  const void* w;
+  int64_t ld_h, ld_w;
+  const float2* part;
+  const void* targets;
+  int target64;
+  int64_t ignore_index;
+  int m, k, v, parts;
+  float* lse;
+  float* loss_rows;
+  float* loss;        // NULL: no sum or mean asked
+  int mean;
+  unsigned* done;
+};
+
+constexpr int kStatsThreads = 128;
+constexpr int kStatsRows = kStatsThreads / 32;
+
+// Joins a row's (max, sum) parts with the target's logit, a warp per row; the
+// CTA that comes last adds the rows' losses up, in row order whichever CTA it
+// is.
+template <typename T>
+__global__ void __launch_bounds__(kStatsThreads) ce_stats(StatsArgs a) {
+  const float ninf = __int_as_float(0xff800000);
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kStatsRows + (threadIdx.x >> 5);
+  const int target = row < a.m ? load_target(a.targets, a.target64, row, a.ignore_index, a.v) : -1;
+  float at = 0.f;
+  if (target >= 0)  // reads only the caller's operands: need not wait for the kernel before
+    at = warp_dot(static_cast<const T*>(a.h) + row * a.ld_h, static_cast<const T*>(a.w) + target * a.ld_w, a.k, lane);
+  pdl_wait();
+  if (row < a.m) {
+    const float2* pr = a.part + row * a.parts;
+    float mx = ninf;
+    for (int i = lane; i < a.parts; i += 32) mx = fmaxf(mx, pr[i].x);
+    mx = warp_max(mx);
+    const float ref = mx == ninf ? 0.f : mx;
+    float sum = 0.f;
+    for (int i = lane; i < a.parts; i += 32) {
+      const float2 t = pr[i];
+      sum += t.y * exp_from(t.x, ref);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      // the log-sum-exp over the words other than the target, and the loss, in
+      // 64 bits: an almost certain target leaves a loss far below the logits'
+      // own rounding
+      const double rest = static_cast<double>(ref) + log(static_cast<double>(sum));
+      double lse = rest, loss = 0.0;
+      if (target >= 0) {
+        const double st = at;
+        const double x = rest - st;
+        loss = x > 0.0 ? x + log1p(exp(-x)) : log1p(exp(x));
+        lse = x > 0.0 ? rest + log1p(exp(-x)) : st + loss;
+        if (st > 3.5e38) loss = lse - st;  // an infinite logit: NaN, as lse - s_t says, not 0
+      } else if (target == -2) {
+        loss = __longlong_as_double(0x7ff8000000000000ll);
+      }
+      a.lse[row] = static_cast<float>(lse);
+      a.loss_rows[row] = static_cast<float>(loss);
+    }
+  }
+  if (!a.loss) return;
+  __shared__ bool last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(a.done, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
   double sum = 0.0;
   int count = 0;
-  for (int i = threadIdx.x; i < m; i += 1024) {
-    sum += static_cast<double>(loss_rows[i]);
-    count += load_target(targets, target64, i, ignore_index, v) != -1;
+  for (int i = threadIdx.x; i < a.m; i += kStatsThreads) {
+    sum += static_cast<double>(__ldcg(a.loss_rows + i));
+    count += load_target(a.targets, a.target64, i, a.ignore_index, a.v) != -1;
   }
-  sum = cta_sum<double, 1024>(sum);
-  count = cta_sum<int, 1024>(count);
-  if (threadIdx.x == 0) *loss = static_cast<float>(mean ? sum / static_cast<double>(count) : sum);
+  sum = cta_sum<double, kStatsThreads>(sum);
+  count = cta_sum<int, kStatsThreads>(count);
+  if (threadIdx.x == 0) *a.loss = static_cast<float>(a.mean ? sum / static_cast<double>(count) : sum);
 }
 
 struct RowsArgs {
@@ -646,7 +1028,7 @@ struct RowsArgs {
   float* row_lse;
   float* row_g;
   float* row_dt;
-  void* hc;           // [m rounded up to 256][k]
+  void* hc;           // [m][k]
 };
 
 constexpr int kRowThreads = 256;
@@ -664,6 +1046,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
   const int r0 = min(a.m, static_cast<int>(blockIdx.x) * per), r1 = min(a.m, r0 + per);
   int before = 0, all = 0;
   float top = 0.f;
+  pdl_wait();
+  pdl_trigger();
   for (int i = tid; i < a.m; i += kRowThreads) {
     if (load_target(a.targets, a.target64, i, a.ignore_index, a.v) == -1) continue;
     all += 1;
@@ -729,11 +1113,38 @@ __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
     }
     __syncthreads();
   }
-  // the rows that fill up the last row tile are contracted over with d = 0: they must be finite
-  const int end = (all + 255) / 256 * 256;
+  // the rows that fill up the last k-block are contracted over with d = 0: they must be finite
+  const int end = min(a.m, (all + BK - 1) / BK * BK);
   for (int r = all + static_cast<int>(blockIdx.x); r < end; r += gridDim.x)
     for (int c = tid; c < packets; c += kRowThreads)
       static_cast<uint4*>(a.hc)[static_cast<int64_t>(r) * packets + c] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// dh = unscale * sum over the splits, in order, for the counted rows. A thread
+// takes 8 columns.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_dh_finish(const float* __restrict__ acc, const RowHeader* header,
+                                                    const int* __restrict__ row_index, int m, int k, int splits, T* dh,
+                                                    int64_t ld_dh) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t groups = static_cast<int64_t>(header->rows) * (k / 8);
+  const float unscale = header->unscale;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < groups; i += gridDim.x * 256ll) {
+    const int64_t row = i / (k / 8);
+    const int col = static_cast<int>(i - row * (k / 8)) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const float4* src = reinterpret_cast<const float4*>(acc + (static_cast<int64_t>(s) * m + row) * k + col);
+      const float4 a = __ldcs(src), b = __ldcs(src + 1);
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= unscale;
+    store8<T>(dh + row_index[row] * ld_dh + col, v);
+  }
 }
 
 // ---- host side -------------------------------------------------------------------------
@@ -761,16 +1172,18 @@ int resident_pairs(cudaLaunchConfig_t cfg) {
 template <int MODE, typename T, typename TW>
 int launch_pair(const char* what, const CeParams& p, int64_t tiles, int max_ctas, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(192, 1, 1);
-  cfg.dynamicSmemBytes = static_cast<size_t>(kStages) * STAGE + 1024 + 256;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.blockDim = dim3(pair_threads(MODE), 1, 1);
+  cfg.dynamicSmemBytes = smem_of(MODE);
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
   int64_t pairs = resident_pairs<MODE, T, TW>(cfg);
   if (pairs <= 0)
     return fail(AXON_E_LAUNCH, "%s: no room for a CTA pair (%s)", what, cudaGetErrorString(cudaGetLastError()));
@@ -780,6 +1193,55 @@ int launch_pair(const char* what, const CeParams& p, int64_t tiles, int max_ctas
   cudaError_t e = cudaLaunchKernelEx(&cfg, ce_pair<MODE, T, TW>, p);
   if (e != cudaSuccess) return fail(AXON_E_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
   return launch_status(what);
+}
+
+template <int MODE, typename T, int NT>
+int launch_narrow_nt(const char* what, const CeParams& p, int grid, cudaStream_t s) {
+  constexpr int smem = narrow_stages(NT) * narrow_stage(NT) + 2048;
+  static bool set[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return fail(AXON_E_CUDA, "%s: no current device", what);
+  auto kern = ce_narrow<MODE, T, NT>;
+  if (!set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(AXON_E_LAUNCH, "%s: smem attribute: %s", what, cudaGetErrorString(e));
+    set[dev] = true;
+  }
+  cudaError_t e = launch_k(kern, dim3(grid), dim3(192), smem, s, p);
+  if (e != cudaSuccess) return fail(AXON_E_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  return launch_status(what);
+}
+
+// The rows a tile of ce_narrow holds.
+int narrow_nt(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
+
+template <int MODE, typename T>
+int launch_narrow(const char* what, const CeParams& p, int grid, cudaStream_t s) {
+  switch (narrow_nt(p.m)) {
+    case 16: return launch_narrow_nt<MODE, T, 16>(what, p, grid, s);
+    case 32: return launch_narrow_nt<MODE, T, 32>(what, p, grid, s);
+    default: return launch_narrow_nt<MODE, T, 64>(what, p, grid, s);
+  }
+}
+
+// Words a tile of ce_narrow: the smallest multiple of 8 that needs no more
+// rounds of tiles than 128 words would, so the last round is as full as the
+// others (32000 words on 148 SMs: 286 tiles of 112 instead of 250 of 128).
+int narrow_words(int64_t v, int max_ctas) {
+  int64_t g = sm_count();
+  if (max_ctas > 0 && max_ctas < g) g = max_ctas;
+  const int64_t rounds = ((v + BM - 1) / BM + g - 1) / g;
+  const int64_t words = (v + rounds * g - 1) / (rounds * g);
+  return static_cast<int>((words + 7) / 8 * 8);
+}
+
+// CTAs of ce_narrow, at most one per SM.
+int narrow_grid(int64_t v, int max_ctas) {
+  const int64_t words = narrow_words(v, max_ctas), tiles = (v + words - 1) / words;
+  int64_t g = sm_count();
+  if (max_ctas > 0 && max_ctas < g) g = max_ctas;
+  return static_cast<int>(tiles < g ? tiles : g);
 }
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -792,32 +1254,42 @@ int band_of(int64_t k) {
 }
 
 struct GradPlan {
-  int64_t rows;      // m rounded up to the row tile
   int64_t piece;     // words a piece
   int64_t pieces;
+  int splits;        // parts of dh's contraction over a piece
   int64_t off_rows, off_hc, off_d, off_acc, bytes;
 };
 
 constexpr int64_t kPieceBytes = 512ll << 20;  // of d
 
 int grad_plan(int64_t m, int64_t k, int64_t v, const axon_tune_t& t, GradPlan& g) {
-  g.rows = round_up(m, 256);
   if (t.split < 0 || t.split % 256) return fail(AXON_E_ARG, "axon_linear_ce_grad: split must be a multiple of 256 words");
   if (t.split > 0) {
     g.piece = t.split;
   } else {
-    int64_t most = kPieceBytes / (2 * (g.rows ? g.rows : 256)) / 256 * 256;
+    int64_t most = kPieceBytes / (2 * (m ? m : 1)) / 256 * 256;
     if (most < 256) most = 256;
     const int64_t pieces = (v + most - 1) / most;
     g.piece = round_up((v + pieces - 1) / pieces, 256);
   }
   if (g.piece > round_up(v, 256)) g.piece = round_up(v, 256);
   g.pieces = (v + g.piece - 1) / g.piece;
+  // A dh tile contracts over the whole piece while a dw tile contracts over the
+  // rows: with few rows, few pairs would work on dh long after the rest. Cut
+  // the contraction so that a part is at most a third of a pair's share, down
+  // to 16 k-blocks. (64 x 2048 x 32000: 174 us uncut; 1001 x 1024 x 50257: 286.)
+  const int64_t cols = (k + BN - 1) / BN, kb_dh = (g.piece + BK - 1) / BK, kb_dw = (m + BK - 1) / BK;
+  const int64_t n_dh = (m + 255) / 256 * cols, n_dw = g.piece / 256 * cols;
+  const int64_t pairs = sm_count() / 2;
+  const int64_t share = (n_dh * (kb_dh + kTileCost) + n_dw * (kb_dw + kTileCost)) / pairs;
+  int64_t part = share / 3 > 16 ? share / 3 : 16;
+  if (part > kb_dh) part = kb_dh;
+  g.splits = static_cast<int>((kb_dh + part - 1) / part);
   g.off_rows = 256;
-  g.off_hc = g.off_rows + round_up(5 * g.rows * 4, 256);
-  g.off_d = g.off_hc + round_up(g.rows * k * 2, 256);
-  g.off_acc = g.off_d + round_up(g.rows * g.piece * 2, 256);
-  g.bytes = g.off_acc + (g.pieces > 1 ? round_up(g.rows * k * 4, 256) : 0);
+  g.off_hc = g.off_rows + round_up(5 * m * 4, 256);
+  g.off_d = g.off_hc + round_up(m * k * 2, 256);
+  g.off_acc = g.off_d + round_up(m * g.piece * 2, 256);
+  g.bytes = g.off_acc + (g.pieces > 1 || g.splits > 1 ? round_up(g.splits * m * k * 4, 256) : 0);
   return AXON_OK;
 }
 
@@ -851,21 +1323,57 @@ int check_head(const char* what, const void* h, const void* w, const void* targe
   return AXON_OK;
 }
 
+// The operand maps of the logits: the wide kernel takes 128 rows of h and 128
+// words a CTA, the narrow one 128 words and all rows.
+int logits_maps(const char* what, CeParams& p, const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype) {
+  int rc;
+  if (p.m > kNarrowRows) {
+    rc = make_map(&p.a, h, dtype, p.k, p.m, ld_h, BK, BM, "h", what);
+    if (!rc) rc = make_map(&p.b, w, dtype, p.k, p.v, ld_w, BK, BH, "w", what);
+  } else {
+    rc = make_map(&p.a, w, dtype, p.k, p.v, ld_w, BK, p.word_tile, "w", what);
+    if (!rc) rc = make_map(&p.b, h, dtype, p.k, p.m, ld_h, BK, narrow_nt(p.m), "h", what);
+  }
+  p.a2 = p.c = p.a;  // not read by these modes (kDlogits' caller sets c)
+  p.b2 = p.b;
+  return rc;
+}
+
+template <int MODE, typename T>
+int launch_logits(const char* what, const CeParams& p, int max_ctas, cudaStream_t s) {
+  if (p.m <= kNarrowRows) return launch_narrow<MODE, T>(what, p, narrow_grid(p.v, max_ctas), s);
+  const int64_t tiles = (p.m + 255ll) / 256 * ((p.v + BN - 1) / BN);
+  return launch_pair<MODE, T, T>(what, p, tiles, max_ctas, s);
+}
+
 template <typename T>
-int run_loss(const CeParams& p, int64_t tiles, int max_ctas, cudaStream_t s) {
-  return launch_pair<kLse, T, T>("axon_linear_ce", p, tiles, max_ctas, s);
+int run_loss(const CeParams& p, const StatsArgs& a, int max_ctas, cudaStream_t s) {
+  const char* what = "axon_linear_ce";
+  int rc = launch_logits<kLse, T>(what, p, max_ctas, s);
+  if (rc) return rc;
+  launch_k(ce_stats<T>, dim3(static_cast<unsigned>((a.m + kStatsRows - 1) / kStatsRows)), dim3(kStatsThreads), 0, s, a);
+  return launch_status(what);
 }
 
 // Both kernels of one piece.
 template <typename T>
-int run_piece(const CeParams& pl, const CeParams& pg, int32_t dw_dtype, int64_t rows, int max_ctas, cudaStream_t s) {
+int run_piece(const CeParams& pl, const CeParams& pg, int32_t dw_dtype, int max_ctas, cudaStream_t s) {
   const char* what = "axon_linear_ce_grad";
-  int rc = launch_pair<kDlogits, T, T>(what, pl, rows / 256 * ((pl.v + BN - 1) / BN), max_ctas, s);
+  int rc = launch_logits<kDlogits, T>(what, pl, max_ctas, s);
   if (rc) return rc;
   const int64_t cols = (pg.k + BN - 1) / BN;
-  const int64_t tiles = cols * ((pg.dh ? rows / 256 : 0) + (pg.dw ? (pg.v + 255) / 256 : 0));
+  const int64_t tiles = cols * ((pg.dh ? (pg.m + 255ll) / 256 * pg.splits : 0) + (pg.dw ? (pg.v + 255) / 256 : 0));
   if (dw_dtype == AXON_F32) return launch_pair<kGrads, T, float>(what, pg, tiles, max_ctas, s);
   return launch_pair<kGrads, T, T>(what, pg, tiles, max_ctas, s);
+}
+
+template <typename T>
+int run_finish(const CeParams& p, cudaStream_t s) {
+  const int64_t groups = static_cast<int64_t>(p.m) * (p.k / 8);
+  const int64_t cap = 8ll * sm_count(), grid = (groups + 255) / 256;
+  launch_k(ce_dh_finish<T>, dim3(static_cast<unsigned>(grid < cap ? grid : cap)), dim3(256), 0, s,
+           static_cast<const float*>(p.acc), p.header, p.row_index, p.m, p.k, p.splits, static_cast<T*>(p.dh), p.ld_dh);
+  return launch_status("axon_linear_ce_grad");
 }
 
 }  // namespace
@@ -878,7 +1386,7 @@ extern "C" {
 int64_t axon_linear_ce_workspace_bytes(int64_t m, int64_t k, int64_t v) {
   int rc = check_sizes("axon_linear_ce", m, k, v);
   if (rc) return rc;
-  return round_up(m * ((v + BN - 1) / BN) * 8, 256) + 256;
+  return 256 + round_up(m * (m > kNarrowRows ? (v + BN - 1) / BN : sm_count()) * 8, 256);
 }
 
 int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse, float* loss_rows, float* loss,
@@ -896,37 +1404,27 @@ int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse
     return fail(AXON_E_ARG, "%s: workspace of %lld bytes needed", what, (long long)need);
   if (!aligned16(workspace)) return fail(AXON_E_ALIGN, "%s: workspace must be 16-byte aligned", what);
   cudaStream_t s = as_stream(stream);
-  const int64_t word_tiles = (v + BN - 1) / BN;
-  if (m > 0) {
-    CeParams p{};
-    if ((rc = make_map(&p.a, h, dtype, k, m, ld_h, BK, BM, "h", what))) return rc;
-    if ((rc = make_map(&p.b, w, dtype, k, v, ld_w, BK, BH, "w", what))) return rc;
-    p.a2 = p.a;
-    p.b2 = p.b;
-    p.m = static_cast<int>(m);
-    p.v = static_cast<int>(v);
-    p.k = static_cast<int>(k);
-    p.targets = targets;
-    p.target64 = target_bits == 64;
-    p.ignore_index = ignore_index;
-    p.part = static_cast<float2*>(workspace);
-    p.band = band_of(k);
-    const int64_t tiles = (m + 255) / 256 * word_tiles;
-    rc = dtype == AXON_BF16 ? run_loss<__nv_bfloat16>(p, tiles, t.max_ctas, s) : run_loss<__half>(p, tiles, t.max_ctas, s);
-    if (rc) return rc;
-    const StatsArgs sa{h, w, ld_h, ld_w, p.part, targets, p.target64, ignore_index, p.m, p.k, p.v,
-                       static_cast<int>(word_tiles), lse, loss_rows};
-    const unsigned grid = static_cast<unsigned>((m + 3) / 4);
-    if (dtype == AXON_BF16) ce_stats<__nv_bfloat16><<<grid, 128, 0, s>>>(sa);
-    else ce_stats<__half><<<grid, 128, 0, s>>>(sa);
-    if ((rc = launch_status(what))) return rc;
+  if (m == 0) {  // no rows: a sum of nothing, a mean of nothing
+    if (reduction == AXON_REDUCE_NONE) return AXON_OK;
+    cudaError_t e = cudaMemsetAsync(loss, reduction == AXON_REDUCE_MEAN ? 0xff : 0, sizeof(float), s);
+    return e == cudaSuccess ? AXON_OK : fail(AXON_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
   }
-  if (reduction != AXON_REDUCE_NONE) {
-    ce_reduce<<<1, 1024, 0, s>>>(loss_rows, targets, target_bits == 64, ignore_index, v, static_cast<int>(m),
-                                 reduction == AXON_REDUCE_MEAN, loss);
-    return launch_status(what);
-  }
-  return AXON_OK;
+  CeParams p{};
+  p.m = static_cast<int>(m);
+  p.v = static_cast<int>(v);
+  p.k = static_cast<int>(k);
+  p.targets = targets;
+  p.target64 = target_bits == 64;
+  p.ignore_index = ignore_index;
+  p.done = static_cast<unsigned*>(workspace);
+  p.part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 256);
+  p.parts = static_cast<int>(m > kNarrowRows ? (v + BN - 1) / BN : narrow_grid(v, t.max_ctas));
+  p.band = band_of(k);
+  p.word_tile = narrow_words(v, t.max_ctas);
+  if ((rc = logits_maps(what, p, h, ld_h, w, ld_w, dtype))) return rc;
+  const StatsArgs a{h, w, ld_h, ld_w, p.part, targets, p.target64, ignore_index, p.m, p.k, p.v, p.parts, lse, loss_rows,
+                    reduction == AXON_REDUCE_NONE ? nullptr : loss, reduction == AXON_REDUCE_MEAN, p.done};
+  return dtype == AXON_BF16 ? run_loss<__nv_bfloat16>(p, a, t.max_ctas, s) : run_loss<__half>(p, a, t.max_ctas, s);
 }
 
 int64_t axon_linear_ce_grad_workspace_bytes(int64_t m, int64_t k, int64_t v, const axon_tune_t* tune) {
@@ -986,13 +1484,13 @@ int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const
   ra.ld_dh = ld_dh;
   ra.header = reinterpret_cast<RowHeader*>(ws);
   ra.row_index = reinterpret_cast<int*>(ws + g.off_rows);
-  ra.row_target = ra.row_index + g.rows;
-  ra.row_lse = reinterpret_cast<float*>(ra.row_target + g.rows);
-  ra.row_g = ra.row_lse + g.rows;
-  ra.row_dt = ra.row_g + g.rows;
+  ra.row_target = ra.row_index + m;
+  ra.row_lse = reinterpret_cast<float*>(ra.row_target + m);
+  ra.row_g = ra.row_lse + m;
+  ra.row_dt = ra.row_g + m;
   ra.hc = ws + g.off_hc;
   const int64_t cap = 4ll * sm_count();
-  ce_grad_rows<<<static_cast<unsigned>(m < cap ? m : cap), kRowThreads, 0, s>>>(ra);
+  launch_k(ce_grad_rows, dim3(static_cast<unsigned>(m < cap ? m : cap)), dim3(kRowThreads), 0, s, ra);
   if ((rc = launch_status(what))) return rc;
 
   for (int64_t i = 0; i < g.pieces; ++i) {
@@ -1019,18 +1517,26 @@ int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const
     p.first = i == 0;
     p.last = i + 1 == g.pieces;
     p.band = band_of(k);
+    p.splits = g.splits;
+    p.word_tile = narrow_words(vc, t.max_ctas);
     CeParams pg = p;
-    if ((rc = make_map(&p.a, ra.hc, dtype, k, g.rows, k, BK, BM, "h", what))) return rc;
-    if ((rc = make_map(&p.b, wp, dtype, k, vc, ld_w, BK, BH, "w", what))) return rc;
-    p.a2 = p.a;
-    p.b2 = p.b;
-    if ((rc = make_map(&pg.a, p.d, dtype, vc, g.rows, p.ld_d, BK, BM, "d", what))) return rc;
+    if ((rc = logits_maps(what, p, ra.hc, k, wp, ld_w, dtype))) return rc;
+    if ((rc = make_map(&p.c, p.d, dtype, vc, m, p.ld_d, 64, 32, "d", what))) return rc;
+    if ((rc = make_map(&pg.a, p.d, dtype, vc, m, p.ld_d, BK, BM, "d", what))) return rc;
     if ((rc = make_map(&pg.b, wp, dtype, k, vc, ld_w, 64, BK, "w", what))) return rc;
-    if ((rc = make_map(&pg.a2, p.d, dtype, vc, g.rows, p.ld_d, 64, BK, "d", what))) return rc;
-    if ((rc = make_map(&pg.b2, ra.hc, dtype, k, g.rows, k, 64, BK, "h", what))) return rc;
-    rc = dtype == AXON_BF16 ? run_piece<__nv_bfloat16>(p, pg, dw_dtype, g.rows, t.max_ctas, s)
-                            : run_piece<__half>(p, pg, dw_dtype, g.rows, t.max_ctas, s);
+    if ((rc = make_map(&pg.a2, p.d, dtype, vc, m, p.ld_d, 64, BK, "d", what))) return rc;
+    if ((rc = make_map(&pg.b2, ra.hc, dtype, k, m, k, 64, BK, "h", what))) return rc;
+    pg.c = pg.a;
+    if (dw) {
+      char* dwp = static_cast<char*>(dw) + v0 * ld_dw * dtype_size(dw_dtype);
+      if ((rc = make_map(&pg.c, dwp, dw_dtype, k, vc, ld_dw, 128 / dtype_size(dw_dtype), 32, "dw", what))) return rc;
+    }
+    rc = dtype == AXON_BF16 ? run_piece<__nv_bfloat16>(p, pg, dw_dtype, t.max_ctas, s)
+                            : run_piece<__half>(p, pg, dw_dtype, t.max_ctas, s);
     if (rc) return rc;
+    if (p.last && dh && g.splits > 1 &&
+        (rc = dtype == AXON_BF16 ? run_finish<__nv_bfloat16>(p, s) : run_finish<__half>(p, s)))
+      return rc;
   }
   return AXON_OK;
 }
