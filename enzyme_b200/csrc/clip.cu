@@ -3,31 +3,34 @@
 //   norm = sqrt(sum over tensors and elements of x^2)
 //   scale = min(1, max_norm / (norm + eps));  y = scale * x
 //
-// The list's tensors are cut into chunks of 16 KB (a chunk never straddles two
-// tensors), numbered through the list, and CTA b of the persistent grid takes
-// the contiguous range [b N / G, (b + 1) N / G): every CTA carries the same
-// bytes whatever the tensors' sizes. The tensor table travels as a kernel
-// argument (no copy to the device, nothing to keep between calls; a captured
-// graph holds it), so a list longer than the table takes several launches.
+// The list's tensors are cut into chunks of 32 KB (a chunk never straddles two
+// tensors), numbered through the list and dealt in turn to the CTAs of a
+// persistent grid: every CTA carries the same bytes whatever the tensors'
+// sizes, and the CTAs move through memory side by side. The tensor table
+// travels as a kernel argument (no copy to the device, nothing to keep
+// between calls; a captured graph holds it), so a list longer than the table
+// takes several launches.
 //
-// Norm: each thread squares and adds 64 bytes of a chunk in fp32 (chains of a
+// Norm: each thread squares and adds 128 bytes of a chunk in fp32 (chains of a
 // few elements), then adds that to a float64 running sum; the CTA's float64
 // partial goes to its own workspace slot, and the slots are added in a fixed
 // order by whoever needs the total: no atomics, the same bits every time.
-// HBM-bound: one read of the gradients.
+// HBM-bound: one read of the gradients. 0.87e9 bf16 gradients: 254 us, 6.9 TB/s
+// (contiguous ranges 259, 16 KB chunks 289).
 //
 // Clip: the norm kernel, then a kernel whose CTAs each add up the slots (a few
-// KB, from L2) and scale their range, walking it backwards: the chunks that
-// the first kernel read last are still in L2.
+// KB, from L2) and scale their chunks, last ones first: what the first kernel
+// read last is still in L2. The same gradients: 850 us, of which three passes
+// at the copy rate are 800.
 #include "common.cuh"
 
 namespace axon {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunkBytes = 16384;
+constexpr int kChunkBytes = 32768;
 constexpr int kVecs = kChunkBytes / 16 / kThreads;  // 16-byte packets a thread takes of a chunk
-constexpr int kCtasPerSm = 6;
+constexpr int kCtasPerSm = 4;
 
 // One launch's share of the list. `first[i]` is tensor i's first chunk within
 // this launch; first[count] the launch's chunk count.
@@ -40,17 +43,6 @@ struct GradTable {
   uint8_t dtype[CAP];
   int32_t count;
 };
-
-template <int CAP>
-__device__ __forceinline__ int find_tensor(const GradTable<CAP>& t, uint32_t chunk) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.first[mid] <= chunk) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
 
 // Sum of v over the CTA in a fixed order, returned to every thread.
 __device__ __forceinline__ double block_sum(double v) {
@@ -144,18 +136,14 @@ __device__ __forceinline__ float chunk_squares(const Chunk& c, int dt) {
 template <int CAP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     grad_squares(const __grid_constant__ GradTable<CAP> t, double* __restrict__ part) {
-  const uint64_t chunks = t.first[t.count];
-  const uint32_t c0 = static_cast<uint32_t>(chunks * blockIdx.x / gridDim.x);
-  const uint32_t c1 = static_cast<uint32_t>(chunks * (blockIdx.x + 1) / gridDim.x);
+  const uint32_t chunks = t.first[t.count];
   pdl_wait();
   double sum = 0.0;
-  if (c0 < c1) {
-    int i = find_tensor(t, c0);
-    for (uint32_t c = c0; c < c1; ++c) {
-      while (c >= t.first[i + 1]) ++i;
-      const int dt = t.dtype[i];
-      sum += static_cast<double>(chunk_squares(chunk_of(t.in[i], t.n[i], dt, c - t.first[i]), dt));
-    }
+  int i = 0;
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+    while (c >= t.first[i + 1]) ++i;
+    const int dt = t.dtype[i];
+    sum += static_cast<double>(chunk_squares(chunk_of(t.in[i], t.n[i], dt, c - t.first[i]), dt));
   }
   pdl_trigger();
   sum = block_sum(sum);
@@ -220,6 +208,8 @@ __device__ __forceinline__ void scale_one(const void* p, void* q, int dt, float 
   else *static_cast<__half*>(q) = __float2half_rn(x);
 }
 
+// STREAM: reads and writes that leave L2 alone (see run_lists).
+template <bool STREAM>
 __device__ __forceinline__ void scale_chunk(const Chunk& c, char* q, int dt, float scale) {
   const int es = dt == AXON_F32 ? 4 : 2;
   if (((reinterpret_cast<uintptr_t>(c.p) ^ reinterpret_cast<uintptr_t>(q)) & 15u) != 0) {
@@ -233,12 +223,15 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, char* q, int dt, flo
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int at = i * kThreads + threadIdx.x;
-    v[i] = at < c.vecs ? __ldcs(src + at) : make_uint4(0u, 0u, 0u, 0u);
+    v[i] = at < c.vecs ? (STREAM ? __ldcs(src + at) : src[at]) : make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int at = i * kThreads + threadIdx.x;
-    if (at < c.vecs) __stcs(dst + at, scale_packet(v[i], dt, scale));
+    if (at >= c.vecs) continue;
+    const uint4 r = scale_packet(v[i], dt, scale);
+    if (STREAM) __stcs(dst + at, r);
+    else dst[at] = r;
   }
   if (threadIdx.x < 16) {
     const int off = edge_offset(c, es, threadIdx.x);
@@ -246,12 +239,10 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, char* q, int dt, flo
   }
 }
 
-template <int CAP>
+template <int CAP, bool STREAM>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     grad_scale(const __grid_constant__ GradTable<CAP> t, ClipArgs a) {
-  const uint64_t chunks = t.first[t.count];
-  const uint32_t c0 = static_cast<uint32_t>(chunks * blockIdx.x / gridDim.x);
-  const uint32_t c1 = static_cast<uint32_t>(chunks * (blockIdx.x + 1) / gridDim.x);
+  const uint32_t chunks = t.first[t.count];
   pdl_wait();
   const float norm = total_norm(a.part, a.parts);
   const float scale = clip_scale(norm, a.max_norm, a.eps);
@@ -259,14 +250,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     if (a.norm) *a.norm = norm;
     if (a.scale) *a.scale = scale;
   }
-  if (c0 >= c1) return;
-  int i = find_tensor(t, c1 - 1);
-  for (uint32_t c = c1; c-- > c0;) {
+  int i = t.count - 1;
+  for (int64_t at = (static_cast<int64_t>(chunks) - 1 - blockIdx.x) / gridDim.x; at >= 0 && blockIdx.x < chunks; --at) {
+    const uint32_t c = static_cast<uint32_t>(at) * gridDim.x + blockIdx.x;
     while (c < t.first[i]) --i;
     if (scale == 1.f && t.in[i] == t.out[i]) continue;  // in place and nothing to clip
     const int dt = t.dtype[i];
     const int64_t local = c - t.first[i];
-    scale_chunk(chunk_of(t.in[i], t.n[i], dt, local), static_cast<char*>(t.out[i]) + local * kChunkBytes, dt, scale);
+    scale_chunk<STREAM>(chunk_of(t.in[i], t.n[i], dt, local), static_cast<char*>(t.out[i]) + local * kChunkBytes, dt, scale);
   }
 }
 
@@ -355,8 +346,16 @@ int run_lists(const char* what, const GradLists& g, ClipArgs a, double* part, cu
     launch_k(grad_norm_finish, dim3(1), dim3(kThreads), 0, s, a);
     return launch_status(what);
   }
+  // Gradients that fit L2 (126 MB) are still there for the second pass if its
+  // writes do not push them out: streaming (66 MB: 29 us, 31 without). Of more
+  // than that little is left, and plain accesses are faster (0.8 GB: 393 us, 403
+  // streaming).
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < g.count; ++i) bytes += g.n[i] * dtype_size(g.dtype[i]);
+  const bool stream = bytes < (126ll << 20);
   return for_each_table<CAP>(g, [&](const GradTable<CAP>& t, int grid) {
-    launch_k(grad_scale<CAP>, dim3(grid), dim3(kThreads), 0, s, t, a);
+    if (stream) launch_k(grad_scale<CAP, true>, dim3(grid), dim3(kThreads), 0, s, t, a);
+    else launch_k(grad_scale<CAP, false>, dim3(grid), dim3(kThreads), 0, s, t, a);
     return launch_status(what);
   });
 }

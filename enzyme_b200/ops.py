@@ -30,7 +30,9 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle torch.cuda.current_stream(t.device).cuda_stream holds, without
+    # the Stream object (2 us of every call)
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _require_cuda(*ts: torch.Tensor | None) -> None:
@@ -280,7 +282,7 @@ class GradList:
                 end_out = max(end_out, hi)
 
     def _ready(self, clip: bool):
-        """(workspace, stream) for a call on this list."""
+        """(results, their address, the workspace's, stream) for a call on this list."""
         if [t.data_ptr() for t in self.grads] != self._where:
             raise N.AxonError(N.AXON_E_ARG, "gradient list: a gradient's memory has moved; make a new GradList")
         if clip:
@@ -291,7 +293,11 @@ class GradList:
                 self._clippable = True
         if self._ws_bytes == 0:
             self._ws_bytes = _check_ws_bytes(N.lib().axon_grad_norm_workspace_bytes(len(self.grads)))
-        return torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device), _stream(self.grads[0])
+        # results in the first two floats, workspace behind them (a few KB): one
+        # allocation of its own for every call, so calls and captured graphs share nothing
+        res = torch.empty(2 + self._ws_bytes // 4, dtype=torch.float32, device=self.device)
+        at = res.data_ptr()
+        return res, at, at + 8, _stream(res)
 
 
 def _grad_list(grads, out=None) -> GradList:
@@ -317,10 +323,9 @@ def grad_norm_scale(grads, max_norm, *, eps=1e-6):
     without rewriting the gradients. A NaN gradient makes both NaN."""
     g = _grad_list(grads)
     with _on_device(g.device):
-        ws, stream = g._ready(clip=False)
-        res = torch.empty(2, dtype=torch.float32, device=g.device)
+        res, at, ws, stream = g._ready(clip=False)
         check(N.lib().axon_grad_norm(g._in_ptrs, g._sizes, g._dtypes, len(g.grads), float(max_norm), float(eps),
-                                     res.data_ptr(), res.data_ptr() + 4, ws.data_ptr(), g._ws_bytes, stream))
+                                     at, at + 4, ws, g._ws_bytes, stream))
     return res[0], res[1]
 
 
@@ -330,11 +335,10 @@ def grad_norm(grads):
     fixed order (the same bits every time)."""
     g = _grad_list(grads)
     with _on_device(g.device):
-        ws, stream = g._ready(clip=False)
-        norm = torch.empty((), dtype=torch.float32, device=g.device)
-        check(N.lib().axon_grad_norm(g._in_ptrs, g._sizes, g._dtypes, len(g.grads), 1.0, 0.0, norm.data_ptr(), None,
-                                     ws.data_ptr(), g._ws_bytes, stream))
-    return norm
+        res, at, ws, stream = g._ready(clip=False)
+        check(N.lib().axon_grad_norm(g._in_ptrs, g._sizes, g._dtypes, len(g.grads), 1.0, 0.0, at, None, ws,
+                                     g._ws_bytes, stream))
+    return res[0]
 
 
 def clip_grads(grads, max_norm, *, eps=1e-6, out=None):
@@ -343,11 +347,10 @@ def clip_grads(grads, max_norm, *, eps=1e-6, out=None):
     default; `out` (or the GradList's) takes the result elsewhere."""
     g = _grad_list(grads, out)
     with _on_device(g.device):
-        ws, stream = g._ready(clip=True)
-        norm = torch.empty((), dtype=torch.float32, device=g.device)
+        res, at, ws, stream = g._ready(clip=True)
         check(N.lib().axon_clip_grads(g._in_ptrs, g._out_ptrs, g._sizes, g._dtypes, len(g.grads), float(max_norm),
-                                      float(eps), norm.data_ptr(), ws.data_ptr(), g._ws_bytes, stream))
-    return g.out, norm
+                                      float(eps), at, ws, g._ws_bytes, stream))
+    return g.out, res[0]
 
 
 def gemm(a, b, *, b2=None, row_scale=None, epilogue=N.AXON_EPI_NONE, out=None, out_dtype=None, tune=None):
@@ -558,14 +561,15 @@ def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", 
     their sum, or their mean over the rows not ignored, in fp32; stats [2, m]
     fp32 holds each row's log-sum-exp and loss, for linear_cross_entropy_grad."""
     m, k, v, ldh, ldw, bits, red = _head_args("linear_cross_entropy", h, w, targets, reduction)
-    stats = torch.empty((2, m), dtype=torch.float32, device=h.device)
-    loss = stats[1] if red == N.AXON_REDUCE_NONE else torch.empty((), dtype=torch.float32, device=h.device)
+    res = torch.empty(2 * m + 1, dtype=torch.float32, device=h.device)
+    stats, at = res.as_strided((2, m), (m, 1)), res.data_ptr()
+    loss = stats[1] if red == N.AXON_REDUCE_NONE else res[2 * m]
     with _on_device(h.device):
         need = _check_ws_bytes(N.lib().axon_linear_ce_workspace_bytes(m, k, v))
         ws = _workspace(need, h.device, workspace)
-        check(N.lib().axon_linear_ce(_ptr(h), _ptr(w), _ptr(targets), stats.data_ptr(), stats.data_ptr() + 4 * m,
-                                     loss.data_ptr(), m, k, v, ldh, ldw, dtype_code(h), bits, int(ignore_index), red,
-                                     ws.data_ptr(), ws.numel(), _tune(tune), _stream(h)))
+        check(N.lib().axon_linear_ce(_ptr(h), _ptr(w), _ptr(targets), at, at + 4 * m, at + 8 * m, m, k, v, ldh, ldw,
+                                     dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.numel(),
+                                     _tune(tune), _stream(h)))
     return loss, stats
 
 
