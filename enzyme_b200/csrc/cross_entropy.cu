@@ -104,7 +104,7 @@ struct CeParams {
   float* acc;           // fp32 [splits][m][k]: dh between pieces, and its splits
   int first, last;      // this piece is the vocabulary's first / last
   int splits;           // parts that dh's contraction over the piece is cut into
-  int word_tile;        // ce_narrow: words a tile
+  int word_tile;        // kLse, kDlogits: words a tile
   int band;             // row tiles of s visited together
 };
 
@@ -166,7 +166,7 @@ struct Walk {
     rows = rows_;
     row_tiles = (rows + 2 * BM - 1) / (2 * BM);
     if constexpr (MODE != kGrads) {
-      word_tiles = (p.v + BN - 1) / BN;
+      word_tiles = (p.v + p.word_tile - 1) / p.word_tile;
       kb_all = (p.k + BK - 1) / BK;
     } else {
       word_tiles = (p.v + 2 * BM - 1) / (2 * BM);
@@ -241,11 +241,11 @@ __device__ __forceinline__ void load_stage(const CeParams& p, const Tile& t, int
   kb += t.k0;
   uint8_t* sb = sa + A_BYTES;
   const int row0 = t.tm * 2 * BM + rank * BM;
-  const int col0 = t.tn * BN + rank * BH;
   if constexpr (MODE != kGrads) {
     tma_load_2d_pair(&p.a, full, sa, kb * BK, row0);
-    tma_load_2d_pair(&p.b, full, sb, kb * BK, col0);
+    tma_load_2d_pair(&p.b, full, sb, kb * BK, t.tn * p.word_tile + rank * (p.word_tile / 2));
   } else {
+    const int col0 = t.tn * BN + rank * BH;
     if (!t.dw) {
       tma_load_2d_pair(&p.a, full, sa, kb * BK, row0);
     } else {
@@ -258,16 +258,25 @@ __device__ __forceinline__ void load_stage(const CeParams& p, const Tile& t, int
   }
 }
 
-// tcgen05 instruction descriptor: fp32 accumulator, M 256, N 256; bit 15 / 16:
+// tcgen05 instruction descriptor: fp32 accumulator, M 256, N columns; bit 15 / 16:
 // A / B is MN-major.
 template <typename T>
-__device__ __forceinline__ uint32_t idesc(bool a_mn, bool b_mn) {
+__device__ __forceinline__ uint32_t idesc(int n, bool a_mn, bool b_mn) {
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
-         (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>((2 * BM) >> 4) << 24);
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>((2 * BM) >> 4) << 24);
 }
 
 // ---- epilogues -----------------------------------------------------------------------
+
+// COLS accumulator columns from tensor memory.
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float* v) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < COLS; i += 32) tmem_ld32(taddr + i, v + i);
+  tmem_wait_ld();
+}
 
 __device__ __forceinline__ float max32(const float* v) {
   float a[8];
@@ -286,13 +295,11 @@ __device__ __forceinline__ void lse_tile(const CeParams& p, const Tile& t, uint3
   const int target = row_ok ? load_target(p.targets, p.target64, row, p.ignore_index, p.v) : -1;
   float mx = ninf, sum = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
-    const int col = t.tn * BN + c * 32;
+  for (int c = 0; c < p.word_tile; c += 32) {
+    const int col = t.tn * p.word_tile + c;
     if (col >= p.v) break;  // the same for the whole warp
     float v[32];
-    __syncwarp();
-    tmem_ld32(tbase + c * 32, v);
-    tmem_wait_ld();
+    tmem_ld_cols<32>(tbase + c, v);
     if (col + 32 > p.v) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
@@ -348,15 +355,6 @@ __device__ __forceinline__ void staging_free(int lane) {
   __syncwarp();
 }
 
-// COLS accumulator columns from tensor memory.
-template <int COLS>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float* v) {
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < COLS; i += 32) tmem_ld32(taddr + i, v + i);
-  tmem_wait_ld();
-}
-
 // This warp is done with the accumulator (its values are in registers).
 __device__ __forceinline__ void release_tmem(uint32_t leader_tempty, int lane) {
   tc_fence_before();
@@ -372,10 +370,12 @@ __device__ __forceinline__ int rows_read(const CeParams& p, int rows) {
   return end < p.m ? end : p.m;
 }
 
-// kDlogits: d for this thread's row in columns [c0, c0 + 128) of the tile. The
-// accumulator is released once its second half is in registers.
+// kDlogits: d for this thread's row in one half of the tile's words, 64 at a
+// time; where that does not divide, the last 64 begin earlier and write some
+// words a second time. The accumulator is released once the last are in
+// registers.
 template <typename T>
-__device__ __forceinline__ void dlogits_tile(const CeParams& p, const Tile& t, uint32_t tbase, int c0, int64_t row0,
+__device__ __forceinline__ void dlogits_tile(const CeParams& p, const Tile& t, uint32_t tbase, int half, int64_t row0,
                                              int lane, int rows, uint8_t* stg, uint32_t tempty) {
   const int64_t row = row0 + lane;
   const bool row_ok = row < rows, any = row0 < rows_read(p, rows);
@@ -384,11 +384,11 @@ __device__ __forceinline__ void dlogits_tile(const CeParams& p, const Tile& t, u
   const float dt = row_ok ? p.row_dt[row] : 0.f;
   const int target = row_ok ? p.row_target[row] - p.v0 : -1;
 #pragma unroll 1
-  for (int c = 0; c < BN / 2; c += 64) {
-    const int col = t.tn * BN + c0 + c;
+  for (int c = 0, words = p.word_tile / 2; c < words; c += 64) {
+    const int at = half * words + (c + 64 > words ? words - 64 : c), col = t.tn * p.word_tile + at;
     float v[64];
-    tmem_ld_cols<64>(tbase + c0 + c, v);
-    if (c + 64 == BN / 2) release_tmem(tempty, lane);
+    tmem_ld_cols<64>(tbase + at, v);
+    if (c + 64 >= words) release_tmem(tempty, lane);
     if (!any || col >= p.v) continue;  // the same for the whole warp
     const int left = row_ok ? p.v - col : 0;  // words of this piece that count
 #pragma unroll
@@ -546,13 +546,14 @@ __global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_co
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
+    const uint32_t pair_bytes = MODE == kGrads ? 2 * STAGE : 2 * A_BYTES + p.word_tile * BK * 2;
     int stage = 0;
     uint32_t phase = 0;
     for (int i = 0; w.at(p, i, t); ++i) {
       for (int kb = 0; kb < t.kb; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_ce_error)) goto producer_done;
         const uint32_t leader_full = mapa_u32(smem_u32(&full[stage]), 0);
-        if (leader) mbar_expect_tx(&full[stage], 2 * STAGE);
+        if (leader) mbar_expect_tx(&full[stage], pair_bytes);
         load_stage<MODE>(p, t, kb, static_cast<int>(rank), smem + stage * STAGE, leader_full);
         *issued += 1;
         if (++stage == kStages) {
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_co
       tc_fence_after();
       const uint32_t d = tmem_base + static_cast<uint32_t>(buf * BN);
       const bool a_mn = MODE == kGrads && t.dw, b_mn = MODE == kGrads;
-      const uint32_t id = idesc<T>(a_mn, b_mn);
+      const uint32_t id = idesc<T>(MODE == kGrads ? BN : p.word_tile, a_mn, b_mn);
       // one K = 16 step: 32 bytes along a K-major row, 16 rows of an MN-major block
       const uint32_t a_step = a_mn ? 2048 : 32, a_lbo = a_mn ? CHUNK : 16;
       const uint32_t b_step = b_mn ? 2048 : 32, b_lbo = b_mn ? CHUNK : 16;
@@ -619,8 +620,8 @@ __global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_co
         release_tmem(leader_tempty, lane);
       } else {
         uint8_t* stg = staging + (warp - 2) * kStaging;
-        const int c0 = warp < 6 ? 0 : BN / 2;  // this warp's half of the columns
-        if constexpr (MODE == kDlogits) dlogits_tile<T>(p, t, tbase, c0, row0, lane, w.rows, stg, leader_tempty);
+        const int half = warp < 6 ? 0 : 1, c0 = half * (BN / 2);  // this warp's half of the columns
+        if constexpr (MODE == kDlogits) dlogits_tile<T>(p, t, tbase, half, row0, lane, w.rows, stg, leader_tempty);
         else if (t.dw) dw_tile<TW>(p, t, tbase, c0, row0, lane, unscale, stg, leader_tempty);
         else dh_tile<T>(p, t, tbase, c0, row0, lane, w.rows, unscale, stg, leader_tempty);
       }
@@ -644,25 +645,34 @@ __global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_co
 
 // ---- few rows: the words on the accumulator's lanes -----------------------------------------
 //
-// With at most 64 rows the products are bound by reading w once, and a tile of
+// With at most 128 rows the products are bound by reading w once, and a tile of
 // 256 rows by 256 words would spend its shared memory and MMA time on rows that
-// are not there. Here the words are the MMA's M (128 a tile, one CTA) and the
-// rows its N (NT = 16, 32 or 64), so a k-block stages 16 KB of w beside 2-8 KB of
-// h, ten to twelve of them deep.
+// are not there. Here the words are the MMA's M (up to 128 a tile, one CTA) and
+// the rows its N (NT = 16 to 128), so a k-block stages 16 KB of w beside 2-16 KB
+// of h, six to twelve of them deep. The words a tile holds are chosen so that
+// all CTAs get the same number of tiles.
 //
 //   kLse      a thread owns a lane, so one word of each of its CTA's tiles, and
 //             keeps a running (max, sum) for every row in registers; the 128
 //             lanes are joined once, at the end, into one (max, sum) per row
 //             and CTA;
 //   kDlogits  a warp's 32 lanes are 32 neighbouring words of a row of d.
-constexpr int kNarrowRows = 64;
+constexpr int kNarrowRows = 128;
 constexpr int kNarrowMaxStages = 12;
 
 constexpr int narrow_stage(int nt) { return A_BYTES + nt * BK * 2; }
-constexpr int narrow_stages(int nt) {
-  const int fit = (232448 - 1024 - 1024) / narrow_stage(nt);
+// Per row: the target (kLse), or what its entries of d need (kDlogits).
+constexpr int narrow_row_bytes(int mode) { return mode == kLse ? 4 : 16; }
+constexpr int narrow_extra(int mode, int nt) { return 1024 + 256 + nt * narrow_row_bytes(mode); }
+constexpr int narrow_stages(int mode, int nt) {
+  const int fit = (232448 - narrow_extra(mode, nt)) / narrow_stage(nt);
   return fit < kNarrowMaxStages ? fit : kNarrowMaxStages;
 }
+constexpr int narrow_smem(int mode, int nt) { return narrow_stages(mode, nt) * narrow_stage(nt) + narrow_extra(mode, nt); }
+// Epilogue warps: each takes 32 of the rows (16 of 16) on its quarter of the lanes.
+constexpr int narrow_cols(int nt) { return nt < 32 ? nt : 32; }
+constexpr int narrow_epi_warps(int nt) { return 4 * nt / narrow_cols(nt); }
+constexpr int narrow_threads(int nt) { return 64 + 32 * narrow_epi_warps(nt); }
 
 // 32 lanes x 16 consecutive 32-bit TMEM columns.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
@@ -685,11 +695,13 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 }
 
 template <int MODE, typename T, int NT>
-__global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CeParams p) {
-  constexpr int S = narrow_stages(NT);
+__global__ void __launch_bounds__(narrow_threads(NT), 1) ce_narrow(const __grid_constant__ CeParams p) {
+  constexpr int S = narrow_stages(MODE, NT);
   constexpr int SB = narrow_stage(NT);
+  constexpr int CW = narrow_cols(NT), EPI = 32 * narrow_epi_warps(NT);
   constexpr uint32_t COLS = 2 * NT < 32 ? 32 : 2 * NT;
-  static_assert(S * SB >= 128 * NT * 8, "the lanes' pairs are joined in the stages' memory");
+  static_assert(S * SB >= 129 * NT * 8, "the lanes' pairs are joined in the stages' memory");
+  static_assert((2 * S + 5) * 8 + 16 <= 256, "the rows' values begin 256 bytes behind the stages");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * SB);
@@ -700,7 +712,8 @@ __global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CePa
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* issued = reinterpret_cast<int*>(tmem_slot + 2);
-  int* row_target = reinterpret_cast<int*>(tmem_slot + 4);  // [NT]
+  int* row_target = reinterpret_cast<int*>(smem + S * SB + 256);       // kLse: [NT]
+  float4* row_value = reinterpret_cast<float4*>(smem + S * SB + 256);  // kDlogits: [NT] lse, g, entry at the target, target
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -710,7 +723,7 @@ __global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CePa
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 4);  // one arrival per epilogue warp
+      mbar_init(&tempty[b], EPI / 32);  // one arrival per epilogue warp
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -728,14 +741,13 @@ __global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CePa
   pdl_wait();
   pdl_trigger();
   const int rows = p.header ? p.header->rows : p.m;
-  if (threadIdx.x < NT) {
-    const int r = threadIdx.x;
-    int t = -1;
-    if (r < rows) {
-      if constexpr (MODE == kLse) t = load_target(p.targets, p.target64, r, p.ignore_index, p.v);
-      else t = p.row_target[r] - p.v0;
-    }
-    row_target[r] = t;
+  for (int r = threadIdx.x; r < NT; r += narrow_threads(NT)) {
+    if constexpr (MODE == kLse)
+      row_target[r] = r < rows ? load_target(p.targets, p.target64, r, p.ignore_index, p.v) : -1;
+    else
+      row_value[r] = r < rows ? make_float4(p.row_lse[r], p.row_g[r], p.row_dt[r],
+                                            __int_as_float(p.row_target[r] - p.v0))
+                              : make_float4(0.f, 0.f, 0.f, __int_as_float(-1));
   }
   if (MODE == kLse && blockIdx.x == 0 && threadIdx.x == 64) *p.done = 0;
   __syncthreads();
@@ -804,15 +816,17 @@ __global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CePa
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
     const float ninf = __int_as_float(0xff800000);
-    const int q = warp & 3;  // TMEM lane quarter this warp may access
-    float mx[MODE == kLse ? NT : 1], sm[MODE == kLse ? NT : 1];
+    const int q = warp & 3;                 // TMEM lane quarter this warp may access
+    const int c0 = (warp - 2) / 4 * CW;     // its first row
+    float mx[MODE == kLse ? CW : 1], sm[MODE == kLse ? CW : 1];
     if constexpr (MODE == kLse) {
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
+      for (int c = 0; c < CW; ++c) {
         mx[c] = ninf;
         sm[c] = 0.f;
       }
     }
+    const int write = MODE == kDlogits ? rows_read(p, rows) : p.m;
     int i = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
       const int buf = i & 1;
@@ -820,30 +834,29 @@ __global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CePa
       tc_fence_after();
       // lanes past the tile's words hold what the stage held before
       const int word = q * 32 + lane < p.word_tile ? t * p.word_tile + q * 32 + lane : 0x7fffffff;
-      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * NT);
-      const int write = MODE == kDlogits ? rows_read(p, rows) : 0;
+      const uint32_t tbase =
+          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * NT + c0);
+      if (c0 < write) {  // the same for the whole warp
 #pragma unroll
-      for (int c0 = 0; c0 < NT; c0 += 16) {
-        if (c0 >= p.m) break;  // the same for the whole warp
-        float v[16];
-        __syncwarp();
-        tmem_ld16(tbase + c0, v);
-        tmem_wait_ld();
+        for (int c1 = 0; c1 < CW; c1 += 16) {
+          float v[16];
+          __syncwarp();
+          tmem_ld16(tbase + c1, v);
+          tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int c = c0 + j;
-          if constexpr (MODE == kLse) {
-            const float x = word < p.v && row_target[c] != word ? v[j] : ninf;
-            const float nm = fmaxf(mx[c], x);
-            const float ref = nm == ninf ? 0.f : nm;
-            sm[c] = sm[c] * exp_from(mx[c], ref) + exp_from(x, ref);
-            mx[c] = nm;
-          } else {
-            if (c < write && word < p.ld_d) {
-              float x = 0.f;
-              if (c < rows && word < p.v)
-                x = row_target[c] == word ? p.row_dt[c] : exp_from(v[j], p.row_lse[c]) * p.row_g[c];
-              static_cast<T*>(p.d)[c * p.ld_d + word] = from_f<T>(x);
+          for (int j = 0; j < 16; ++j) {
+            const int c = c1 + j;
+            if constexpr (MODE == kLse) {
+              const float x = word < p.v && row_target[c0 + c] != word ? v[j] : ninf;
+              const float nm = fmaxf(mx[c], x);
+              const float ref = nm == ninf ? 0.f : nm;
+              sm[c] = sm[c] * exp_from(mx[c], ref) + exp_from(x, ref);
+              mx[c] = nm;
+            } else {
+              const float4 r = row_value[c0 + c];
+              float x = __float_as_int(r.w) == word ? r.z : exp_from(v[j], r.x) * r.y;
+              if (word >= p.v || c0 + c >= rows) x = 0.f;
+              if (c0 + c < write && word < p.ld_d) static_cast<T*>(p.d)[(c0 + c) * p.ld_d + word] = from_f<T>(x);
             }
           }
         }
@@ -854,29 +867,27 @@ __global__ void __launch_bounds__(192, 1) ce_narrow(const __grid_constant__ CePa
     }
     if constexpr (MODE == kLse) {
       // every stage has been read (the last accumulator is done): its memory
-      // takes the lanes' pairs, a row of NT per lane
+      // takes the lanes' pairs, 128 (and one of padding) for each row
       float2* lanes = reinterpret_cast<float2*>(smem);
-      const int l = q * 32 + lane;
+      const int e = threadIdx.x - 64;
 #pragma unroll
-      for (int c = 0; c < NT; ++c) lanes[l * NT + c] = make_float2(mx[c], sm[c]);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      constexpr int SEG = 128 / NT;  // threads that share a row
-      const int c = l % NT, seg = l / NT;
+      for (int c = 0; c < CW; ++c) lanes[(c0 + c) * 129 + q * 32 + lane] = make_float2(mx[c], sm[c]);
+      asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
+      constexpr int SEG = EPI / NT, PER = 128 / SEG;  // threads that share a row, lanes each
+      const float2* mine = lanes + (e % NT) * 129 + e / NT * PER;
       float2 s = make_float2(ninf, 0.f);
 #pragma unroll 16
-      for (int j = 0; j < NT; ++j) s.x = fmaxf(s.x, lanes[(seg * NT + j) * NT + c].x);
+      for (int j = 0; j < PER; ++j) s.x = fmaxf(s.x, mine[j].x);
       const float ref = s.x == ninf ? 0.f : s.x;
 #pragma unroll 16
-      for (int j = 0; j < NT; ++j) {
-        const float2 o = lanes[(seg * NT + j) * NT + c];
-        s.y += o.y * exp_from(o.x, ref);
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      lanes[l] = s;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (l < rows) {
-        for (int j = 1; j < SEG; ++j) s = join(s, lanes[j * NT + l]);
-        p.part[static_cast<int64_t>(l) * p.parts + blockIdx.x] = s;
+      for (int j = 0; j < PER; ++j) s.y += mine[j].y * exp_from(mine[j].x, ref);
+      asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
+      lanes[e] = s;
+      asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
+      if (e < rows) {  // NT threads at most: rows <= NT
+#pragma unroll
+        for (int j = 1; j < SEG; ++j) s = join(s, lanes[j * NT + e]);
+        p.part[static_cast<int64_t>(e) * p.parts + blockIdx.x] = s;
       }
     }
   }
@@ -968,22 +979,24 @@ __global__ void __launch_bounds__(kStatsThreads) ce_stats(StatsArgs a) {
     }
     sum = warp_sum(sum);
     if (lane == 0) {
-      // the log-sum-exp over the words other than the target, and the loss, in
-      // 64 bits: an almost certain target leaves a loss far below the logits'
-      // own rounding
-      const double rest = static_cast<double>(ref) + log(static_cast<double>(sum));
-      double lse = rest, loss = 0.0;
+      const float rest = ref + logf(sum);  // the log-sum-exp over the words other than the target
+      float lse = rest, loss = 0.f;
       if (target >= 0) {
-        const double st = at;
-        const double x = rest - st;
-        loss = x > 0.0 ? x + log1p(exp(-x)) : log1p(exp(x));
-        lse = x > 0.0 ? rest + log1p(exp(-x)) : st + loss;
-        if (st > 3.5e38) loss = lse - st;  // an infinite logit: NaN, as lse - s_t says, not 0
+        // loss = log(1 + y) with y the other words' odds against the target, so
+        // that an almost certain target's loss keeps its digits; past e^80, log y
+        const float x = ref - at;
+        if (x > 80.f) {
+          loss = x + logf(sum);
+        } else {
+          loss = log1pf(sum * expf(x));
+          lse = at + loss;
+        }
+        if (at > 3.4e38f) loss = lse - at;  // an infinite logit: NaN, as lse - s_t says, not 0
       } else if (target == -2) {
-        loss = __longlong_as_double(0x7ff8000000000000ll);
+        loss = __int_as_float(0x7fc00000);
       }
-      a.lse[row] = static_cast<float>(lse);
-      a.loss_rows[row] = static_cast<float>(loss);
+      a.lse[row] = lse;
+      a.loss_rows[row] = loss;
     }
   }
   if (!a.loss) return;
@@ -1120,8 +1133,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
       static_cast<uint4*>(a.hc)[static_cast<int64_t>(r) * packets + c] = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// dh = unscale * sum over the splits, in order, for the counted rows. A thread
-// takes 8 columns.
+// dh = unscale * sum over the splits for the counted rows. Four lanes share 8
+// columns, each adding every fourth split in order, and are joined in order.
 template <typename T>
 __global__ void __launch_bounds__(256) ce_dh_finish(const float* __restrict__ acc, const RowHeader* header,
                                                     const int* __restrict__ row_index, int m, int k, int splits, T* dh,
@@ -1130,20 +1143,28 @@ __global__ void __launch_bounds__(256) ce_dh_finish(const float* __restrict__ ac
   pdl_trigger();
   const int64_t groups = static_cast<int64_t>(header->rows) * (k / 8);
   const float unscale = header->unscale;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < groups; i += gridDim.x * 256ll) {
-    const int64_t row = i / (k / 8);
-    const int col = static_cast<int>(i - row * (k / 8)) * 8;
+  const int part = threadIdx.x & 3;
+  // all lanes of a warp take the same number of rounds: they exchange sums
+  for (int64_t i0 = blockIdx.x * 64ll; i0 < groups; i0 += gridDim.x * 64ll) {
+    const int64_t i = i0 + (threadIdx.x >> 2);
+    const bool ok = i < groups;
+    const int64_t row = ok ? i / (k / 8) : 0;
+    const int col = ok ? static_cast<int>(i - row * (k / 8)) * 8 : 0;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
+#pragma unroll 8
+    for (int s = part; s < splits; s += 4) {
       const float4* src = reinterpret_cast<const float4*>(acc + (static_cast<int64_t>(s) * m + row) * k + col);
       const float4 a = __ldcs(src), b = __ldcs(src + 1);
       v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
       v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= unscale;
-    store8<T>(dh + row_index[row] * ld_dh + col, v);
+    for (int e = 0; e < 8; ++e) {
+      v[e] += __shfl_xor_sync(0xffffffffu, v[e], 1);
+      v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
+      v[e] *= unscale;
+    }
+    if (ok && part == 0) store8<T>(dh + row_index[row] * ld_dh + col, v);
   }
 }
 
@@ -1197,7 +1218,7 @@ int launch_pair(const char* what, const CeParams& p, int64_t tiles, int max_ctas
 
 template <int MODE, typename T, int NT>
 int launch_narrow_nt(const char* what, const CeParams& p, int grid, cudaStream_t s) {
-  constexpr int smem = narrow_stages(NT) * narrow_stage(NT) + 2048;
+  constexpr int smem = narrow_smem(MODE, NT);
   static bool set[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
@@ -1208,21 +1229,40 @@ int launch_narrow_nt(const char* what, const CeParams& p, int grid, cudaStream_t
     if (e != cudaSuccess) return fail(AXON_E_LAUNCH, "%s: smem attribute: %s", what, cudaGetErrorString(e));
     set[dev] = true;
   }
-  cudaError_t e = launch_k(kern, dim3(grid), dim3(192), smem, s, p);
+  cudaError_t e = launch_k(kern, dim3(grid), dim3(narrow_threads(NT)), smem, s, p);
   if (e != cudaSuccess) return fail(AXON_E_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
   return launch_status(what);
 }
 
 // The rows a tile of ce_narrow holds.
-int narrow_nt(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
+int narrow_nt(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
 
 template <int MODE, typename T>
 int launch_narrow(const char* what, const CeParams& p, int grid, cudaStream_t s) {
   switch (narrow_nt(p.m)) {
     case 16: return launch_narrow_nt<MODE, T, 16>(what, p, grid, s);
     case 32: return launch_narrow_nt<MODE, T, 32>(what, p, grid, s);
-    default: return launch_narrow_nt<MODE, T, 64>(what, p, grid, s);
+    case 64: return launch_narrow_nt<MODE, T, 64>(what, p, grid, s);
+    default: return launch_narrow_nt<MODE, T, 128>(what, p, grid, s);
   }
+}
+
+// Words a tile of ce_pair: the width, of 256 down to 128 in steps of 32, whose
+// rounds of tiles take the least time (a k-block costs about 32 words more than
+// its own): a narrower tile where the last round would be mostly empty (256 x
+// 2048 x 32000: two rounds of 224 words instead of 256).
+int wide_words(int64_t m, int64_t v) {
+  const int64_t pairs = sm_count() / 2, row_tiles = (m + 255) / 256;
+  int best = BN;
+  int64_t least = INT64_MAX;
+  for (int words = BN; words >= 128; words -= 32) {
+    const int64_t rounds = (row_tiles * ((v + words - 1) / words) + pairs - 1) / pairs;
+    if (rounds * (words + 32) < least) {
+      least = rounds * (words + 32);
+      best = words;
+    }
+  }
+  return best;
 }
 
 // Words a tile of ce_narrow: the smallest multiple of 8 that needs no more
@@ -1242,6 +1282,10 @@ int narrow_grid(int64_t v, int max_ctas) {
   int64_t g = sm_count();
   if (max_ctas > 0 && max_ctas < g) g = max_ctas;
   return static_cast<int>(tiles < g ? tiles : g);
+}
+
+int logits_words(int64_t m, int64_t v, int max_ctas) {
+  return m > kNarrowRows ? wide_words(m, v) : narrow_words(v, max_ctas);
 }
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -1329,7 +1373,7 @@ int logits_maps(const char* what, CeParams& p, const void* h, int64_t ld_h, cons
   int rc;
   if (p.m > kNarrowRows) {
     rc = make_map(&p.a, h, dtype, p.k, p.m, ld_h, BK, BM, "h", what);
-    if (!rc) rc = make_map(&p.b, w, dtype, p.k, p.v, ld_w, BK, BH, "w", what);
+    if (!rc) rc = make_map(&p.b, w, dtype, p.k, p.v, ld_w, BK, p.word_tile / 2, "w", what);
   } else {
     rc = make_map(&p.a, w, dtype, p.k, p.v, ld_w, BK, p.word_tile, "w", what);
     if (!rc) rc = make_map(&p.b, h, dtype, p.k, p.m, ld_h, BK, narrow_nt(p.m), "h", what);
@@ -1342,7 +1386,7 @@ int logits_maps(const char* what, CeParams& p, const void* h, int64_t ld_h, cons
 template <int MODE, typename T>
 int launch_logits(const char* what, const CeParams& p, int max_ctas, cudaStream_t s) {
   if (p.m <= kNarrowRows) return launch_narrow<MODE, T>(what, p, narrow_grid(p.v, max_ctas), s);
-  const int64_t tiles = (p.m + 255ll) / 256 * ((p.v + BN - 1) / BN);
+  const int64_t tiles = (p.m + 255ll) / 256 * ((p.v + p.word_tile - 1) / p.word_tile);
   return launch_pair<MODE, T, T>(what, p, tiles, max_ctas, s);
 }
 
@@ -1370,7 +1414,7 @@ int run_piece(const CeParams& pl, const CeParams& pg, int32_t dw_dtype, int max_
 template <typename T>
 int run_finish(const CeParams& p, cudaStream_t s) {
   const int64_t groups = static_cast<int64_t>(p.m) * (p.k / 8);
-  const int64_t cap = 8ll * sm_count(), grid = (groups + 255) / 256;
+  const int64_t cap = 8ll * sm_count(), grid = (groups + 63) / 64;
   launch_k(ce_dh_finish<T>, dim3(static_cast<unsigned>(grid < cap ? grid : cap)), dim3(256), 0, s,
            static_cast<const float*>(p.acc), p.header, p.row_index, p.m, p.k, p.splits, static_cast<T*>(p.dh), p.ld_dh);
   return launch_status("axon_linear_ce_grad");
@@ -1386,7 +1430,8 @@ extern "C" {
 int64_t axon_linear_ce_workspace_bytes(int64_t m, int64_t k, int64_t v) {
   int rc = check_sizes("axon_linear_ce", m, k, v);
   if (rc) return rc;
-  return 256 + round_up(m * (m > kNarrowRows ? (v + BN - 1) / BN : sm_count()) * 8, 256);
+  const int64_t words = wide_words(m, v);
+  return 256 + round_up(m * (m > kNarrowRows ? (v + words - 1) / words : sm_count()) * 8, 256);
 }
 
 int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse, float* loss_rows, float* loss,
@@ -1418,9 +1463,9 @@ int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse
   p.ignore_index = ignore_index;
   p.done = static_cast<unsigned*>(workspace);
   p.part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 256);
-  p.parts = static_cast<int>(m > kNarrowRows ? (v + BN - 1) / BN : narrow_grid(v, t.max_ctas));
+  p.word_tile = logits_words(m, v, t.max_ctas);
+  p.parts = static_cast<int>(m > kNarrowRows ? (v + p.word_tile - 1) / p.word_tile : narrow_grid(v, t.max_ctas));
   p.band = band_of(k);
-  p.word_tile = narrow_words(v, t.max_ctas);
   if ((rc = logits_maps(what, p, h, ld_h, w, ld_w, dtype))) return rc;
   const StatsArgs a{h, w, ld_h, ld_w, p.part, targets, p.target64, ignore_index, p.m, p.k, p.v, p.parts, lse, loss_rows,
                     reduction == AXON_REDUCE_NONE ? nullptr : loss, reduction == AXON_REDUCE_MEAN, p.done};
@@ -1518,7 +1563,7 @@ int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const
     p.last = i + 1 == g.pieces;
     p.band = band_of(k);
     p.splits = g.splits;
-    p.word_tile = narrow_words(vc, t.max_ctas);
+    p.word_tile = logits_words(m, vc, t.max_ctas);
     CeParams pg = p;
     if ((rc = logits_maps(what, p, ra.hc, k, wp, ld_w, dtype))) return rc;
     if ((rc = make_map(&p.c, p.d, dtype, vc, m, p.ld_d, 64, 32, "d", what))) return rc;
