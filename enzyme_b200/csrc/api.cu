@@ -84,6 +84,13 @@ static const char* kVariants[][2] = {
      "{\"id\":3,\"name\":\"balanced_ranges\",\"knobs\":{\"stages\":[0,2,3,4,6],\"block_k\":[0,16,32],\"max_ctas\":[0]}}]}"},
     {"adam",
      "{\"op\":\"adam\",\"variants\":[{\"id\":0,\"name\":\"grid_stride_vec\",\"knobs\":{\"threads\":[0,128,256,512]}}]}"},
+    {"grad_norm",
+     "{\"op\":\"grad_norm\",\"variants\":[{\"id\":0,\"name\":\"chunked_list\",\"knobs\":{}}]}"},
+    {"linear_ce",
+     "{\"op\":\"linear_ce\",\"variants\":[{\"id\":0,\"name\":\"auto\",\"knobs\":{\"max_ctas\":[0]}}]}"},
+    {"linear_ce_grad",
+     "{\"op\":\"linear_ce_grad\",\"variants\":[{\"id\":0,\"name\":\"auto\",\"knobs\":{\"max_ctas\":[0],"
+     "\"split\":[0,8192,16384,32768,65536]}}]}"},
     {"gemm",
      "{\"op\":\"gemm\",\"variants\":[{\"id\":0,\"name\":\"auto\",\"knobs\":{}},"
      "{\"id\":1,\"name\":\"tcgen05_ws_persistent\",\"knobs\":{\"block_m\":[0,128],"

@@ -1390,6 +1390,30 @@ int launch_logits(const char* what, const CeParams& p, int max_ctas, cudaStream_
   return launch_pair<MODE, T, T>(what, p, tiles, max_ctas, s);
 }
 
+// Memory spans of an operand, [begin, end).
+struct Span {
+  const char* name;
+  uintptr_t begin, end;
+};
+
+Span span(const char* name, const void* p, int64_t rows, int64_t ld, int64_t cols, int64_t item) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  return {name, at, p && rows > 0 ? at + static_cast<uintptr_t>(((rows - 1) * ld + cols) * item) : at};
+}
+
+// Outputs may overlap nothing: they are written while the operands are read.
+int check_apart(const char* what, const Span* outs, int n_outs, const Span* ins, int n_ins) {
+  for (int i = 0; i < n_outs; ++i) {
+    for (int j = 0; j < n_ins; ++j)
+      if (outs[i].begin < ins[j].end && ins[j].begin < outs[i].end)
+        return fail(AXON_E_ARG, "%s: %s overlaps %s", what, outs[i].name, ins[j].name);
+    for (int j = 0; j < i; ++j)
+      if (outs[i].begin < outs[j].end && outs[j].begin < outs[i].end)
+        return fail(AXON_E_ARG, "%s: %s overlaps %s", what, outs[i].name, outs[j].name);
+  }
+  return AXON_OK;
+}
+
 template <typename T>
 int run_loss(const CeParams& p, const StatsArgs& a, int max_ctas, cudaStream_t s) {
   const char* what = "axon_linear_ce";
@@ -1497,6 +1521,12 @@ int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const
   if ((dh && ld_dh % 8) || (dw && ld_dw % 8))
     return fail(AXON_E_ALIGN, "%s: leading dimensions must be multiples of 8", what);
   if (!aligned16(dh) || !aligned16(dw)) return fail(AXON_E_ALIGN, "%s: outputs must be 16-byte aligned", what);
+  const Span outs[2] = {span("dh", dh, m, ld_dh, k, 2), span("dw", dw, v, ld_dw, k, dtype_size(dw_dtype))};
+  const Span ins[6] = {span("h", h, m, ld_h, k, 2),   span("w", w, v, ld_w, k, 2),
+                       span("targets", targets, m, 1, 1, target_bits / 8), span("lse", lse, m, 1, 1, 4),
+                       span("loss_rows", loss_rows, m, 1, 1, 4),
+                       span("dloss", dloss, reduction == AXON_REDUCE_NONE ? m : 1, 1, 1, 4)};
+  if ((rc = check_apart(what, outs, 2, ins, 6))) return rc;
   cudaStream_t s = as_stream(stream);
   if (m == 0) {  // no rows: dw is zero
     if (!dw) return AXON_OK;

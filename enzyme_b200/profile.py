@@ -189,6 +189,48 @@ def case_tp_step(gen):
     return lambda: f.forward(x)
 
 
+def _head(gen, m, v, k=4096):
+    h = _randn(m, k, gen=gen)
+    w = _randn(v, k, scale=1.3 / math.sqrt(k), gen=gen)
+    return h, w, torch.randint(0, v, (m,), device="cuda", generator=gen)
+
+
+def case_linear_ce(gen):
+    """ce_pair<0> and ce_stats: loss of 2048 rows, k 4096, v 65536 (0.5 GB of w)."""
+    from . import ops
+
+    h, w, t = _head(gen, 2048, 65536)
+    return lambda: ops.linear_cross_entropy(h, w, t)
+
+
+def case_linear_ce_grad(gen):
+    """ce_grad_rows, ce_pair<1> (d) and ce_pair<2> (both products): gradients of
+    2048 rows, k 4096, v 65536."""
+    from . import ops
+
+    h, w, t = _head(gen, 2048, 65536)
+    _, stats = ops.linear_cross_entropy(h, w, t)
+    one = torch.ones(1, device="cuda")
+    return lambda: ops.linear_cross_entropy_grad(h, w, t, stats, one)
+
+
+def case_linear_ce_token(gen):
+    """ce_narrow: one row against 128256 words of 4096 (1.05 GB streamed)."""
+    from . import ops
+
+    h, w, t = _head(gen, 1, 128256)
+    return lambda: ops.linear_cross_entropy(h, w, t)
+
+
+def case_grad_clip(gen):
+    """grad_squares and grad_scale: 0.27e9 bf16 gradients in two tensors (0.5 GB)."""
+    from . import ops
+
+    grads = [_randn(128 << 20, scale=1e-3, gen=gen) for _ in range(2)]
+    lst = ops.GradList(grads, out=[torch.empty_like(t) for t in grads])
+    return lambda: ops.clip_grads(lst, 1.0)
+
+
 CASES = {
     "adam": (case_adam, "adam_vec"),
     "cast": (case_cast, "cast_vec"),
@@ -202,6 +244,10 @@ CASES = {
     "rmsnorm_matmul": (case_rmsnorm_matmul, "gemm_tcgen05"),
     "softmax_long": (case_softmax_long, "row_streaming_kernel"),
     "softmax_cta": (case_softmax_cta, "row_cta_bulk_kernel"),
+    "linear_ce": (case_linear_ce, "ce_pair"),
+    "linear_ce_grad": (case_linear_ce_grad, "ce_pair"),
+    "linear_ce_token": (case_linear_ce_token, "ce_narrow"),
+    "grad_clip": (case_grad_clip, "grad_scale"),
     "tp_slabs": (case_tp_slabs, "tp_reduce_push_kernel"),
     "tp_step": (case_tp_step, "swiglu_fused_pair"),
 }
@@ -228,6 +274,7 @@ def main(argv=None) -> int:
     torch.cuda.synchronize()
     ops.gemm_status()
     ops.row_status()
+    ops.linear_cross_entropy_status()
     print(f"profile case {args.case}: {args.launches} launches ok")
     return 0
 

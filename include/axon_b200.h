@@ -348,7 +348,8 @@ AXON_API int axon_linear_ce(const void* h, const void* w, const void* targets, f
  * dloss[0] (SUM) or dloss[0] / counted rows (MEAN), dloss fp32 on the device,
  *   d_ij = g_i (exp(s_ij - lse_i) - [j = targets[i]]), dh = d w, dw = d^T h.
  * lse and loss_rows are axon_linear_ce's. dh [m, k] (ld_dh) has h's type, dw
- * [v, k] (ld_dw) w's or AXON_F32; either may be NULL. Both are overwritten.
+ * [v, k] (ld_dw) w's or AXON_F32; either may be NULL. Both are overwritten;
+ * their memory may overlap no operand's and not each other's.
  * The logits are formed again, a piece of the vocabulary at a time:
  * tune->split words a piece (a multiple of 256; 0: as many as keep the
  * piece's d, 16-bit [m, piece], within 512 MB). d is rounded to the operand

@@ -109,6 +109,30 @@ def attention(q, k_t, v):
     return (e / e.sum(axis=1, keepdims=True)) @ _f(v)
 
 
+def linear_cross_entropy(h, w, targets, ignore_index=-100):
+    """Summed softmax cross entropy of the logits h @ w.T and its gradients
+    (loss, dh, dw); rows whose target is `ignore_index` count for nothing."""
+    h, w = _f(h), _f(w)
+    targets = np.asarray(targets)
+    keep = np.flatnonzero(targets != ignore_index)
+    hk, t = h[keep], targets[keep]
+    s = hk @ w.T
+    s = s - s.max(axis=1, keepdims=True)
+    lse = np.log(np.exp(s).sum(axis=1))
+    rows = np.arange(len(keep))
+    d = np.exp(s - lse[:, None])
+    d[rows, t] -= 1.0
+    dh = np.zeros_like(h)
+    dh[keep] = d @ w
+    return np.sum(lse - s[rows, t]), dh, d.T @ hk
+
+
+def grad_scale(grads, max_norm, eps=1e-6):
+    """(norm, scale) of a list of gradients clipped to `max_norm`."""
+    norm = np.sqrt(sum(np.sum(_f(g) ** 2) for g in grads))
+    return norm, min(1.0, max_norm / (norm + eps))
+
+
 # spec name -> oracle over the spec's positional inputs
 ORACLES = {
     "rmsnorm": rmsnorm_sum,

@@ -52,7 +52,8 @@ def _fwd(**kw):
 
 
 def _bwd(**kw):
-    a = dict(h=FAKE, w=FAKE, t=FAKE, lse=FAKE, rows=FAKE, dloss=FAKE, dh=FAKE, dw=FAKE, m=4, k=64, v=100, ldh=64,
+    a = dict(h=FAKE, w=FAKE, t=FAKE, lse=FAKE, rows=FAKE, dloss=FAKE, dh=ctypes.c_void_p(0x7000000),
+             dw=ctypes.c_void_p(0x8000000), m=4, k=64, v=100, ldh=64,
              ldw=64, lddh=64, lddw=64, dt=N.AXON_BF16, dwt=N.AXON_BF16, bits=64, red=N.AXON_REDUCE_MEAN, ws=FAKE,
              wsb=BIG, tune=None)
     a.update(kw)
@@ -92,6 +93,27 @@ def test_more_refusals():
                      (dict(tune=ctypes.byref(N.Tune(split=100))), N.AXON_E_ARG),
                      (dict(ws=ctypes.c_void_p(0x10080)), N.AXON_E_ALIGN)):
         assert _bwd(**kw) == code, (kw, N.last_error())
+
+
+def test_outputs_over_operands_are_refused():
+    """dh and dw are written while the operands are read. Addresses far apart
+    for everything but the pair under test (nothing is dereferenced)."""
+    far = {n: ctypes.c_void_p(0x1000000 * (i + 1)) for i, n in
+           enumerate(("h", "w", "t", "lse", "rows", "dloss", "dh", "dw"))}
+    for out in ("dh", "dw"):
+        for other in far:
+            if other != out:
+                assert _bwd(**{**far, out: far[other], "ws": None}) == N.AXON_E_ARG
+                assert "overlaps" in N.last_error(), N.last_error()
+    assert _bwd(**{**far, "dh": ctypes.c_void_p(0x1000000 + 3 * 64 * 2)}) == N.AXON_E_ARG  # h's last row
+    assert _bwd(**{**far, "ws": None}) == N.AXON_E_ARG and "workspace" in N.last_error()
+
+
+def test_variants_are_listed():
+    import json
+
+    for op in ("linear_ce", "linear_ce_grad", "grad_norm"):
+        assert json.loads(N.variants(op))["op"] == op
 
 
 def test_workspaces():
@@ -493,3 +515,5 @@ def test_wrapper_refusals(cuda_device):
     assert code(lambda: grad(h, w, t, stats, one, dw_dtype=torch.float16)) == N.AXON_E_ARG
     assert code(lambda: grad(h, w, t, stats, one, tune={"split": 100})) == N.AXON_E_ARG
     assert code(lambda: grad(h, w, t, stats, one, out=(h[:2], w))) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one, out=(h, torch.empty_like(w)))) == N.AXON_E_ARG
+    assert code(lambda: grad(h, w, t, stats, one, out=(torch.empty_like(h), w))) == N.AXON_E_ARG
