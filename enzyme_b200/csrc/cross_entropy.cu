@@ -33,8 +33,11 @@
 // number on the device, so ignored rows cost nothing and whatever they hold
 // (NaN, infinities) reaches nothing.
 //
-// f16: d is held times a power of two that puts the largest |g| near 2^14, so
-// that small probabilities are not lost below 2^-24; the epilogues undo it.
+// d is held with g scaled so that the largest |g| is 1 (f16: 2^14), and the
+// epilogues of the products undo it in fp32. So the rounding of d is that of p and
+// p_t - 1, not one that a common g (1 / rows, for the mean) would give every row
+// alike, off by up to half a step of the type in one direction; and in f16
+// probabilities down to 2^-28 keep their digits.
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -72,7 +75,7 @@ constexpr int smem_of(int mode) { return stages_of(mode) * STAGE + staging_of(mo
 // What ce_grad_rows hands to the kernels after it.
 struct RowHeader {
   int rows;         // rows that count
-  float unscale;    // 1 / the power of two that d carries
+  float unscale;    // what d must be multiplied by
 };
 
 struct CeParams {
@@ -1047,8 +1050,8 @@ struct RowsArgs {
 constexpr int kRowThreads = 256;
 
 // Moves the rows that count to the front. Every CTA owns a range of rows; it
-// finds the number of counted rows before its own (and, for f16, the largest
-// |g|) by reading all targets itself: m is at most some ten thousands, and a
+// finds the number of counted rows before its own, and the largest |g|, by
+// reading all targets itself: m is at most some ten thousands, and a
 // second launch would cost more.
 __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
   __shared__ int slot[kRowThreads];
@@ -1065,25 +1068,20 @@ __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
     if (load_target(a.targets, a.target64, i, a.ignore_index, a.v) == -1) continue;
     all += 1;
     before += i < r0;
-    if (a.f16) top = fmaxf(top, fabsf(a.dloss[a.per_row ? i : 0]));
+    top = fmaxf(top, fabsf(a.dloss[a.per_row ? i : 0]));
   }
   before = cta_sum<int, kRowThreads>(before);
   all = cta_sum<int, kRowThreads>(all);
-  float scale = 1.f;
-  if (a.f16) {
-    top = warp_max(top);
-    if (lane == 0) warp_top[warp] = top;
-    __syncthreads();
-    for (int i = 0; i < kRowThreads / 32; ++i) top = fmaxf(top, warp_top[i]);
-    if (a.mean) top /= static_cast<float>(all);
-    if (top > 0.f && top < __int_as_float(0x7f800000)) {
-      // 2^(14 - floor(log2 top)), kept where it and its inverse are normal numbers
-      int e = 14 - ilogbf(top);
-      e = max(-126, min(126, e));
-      scale = ldexpf(1.f, e);
-    }
+  top = warp_max(top);
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+  for (int i = 0; i < kRowThreads / 32; ++i) top = fmaxf(top, warp_top[i]);
+  const float unit = a.f16 ? 16384.f : 1.f;  // what the largest |g| becomes
+  const bool scaled = top > 0.f && top < __int_as_float(0x7f800000);
+  if (blockIdx.x == 0 && tid == 0) {
+    const float weight = a.mean ? 1.f / static_cast<float>(all) : 1.f;
+    *a.header = RowHeader{all, scaled ? top / unit * weight : weight};
   }
-  if (blockIdx.x == 0 && tid == 0) *a.header = RowHeader{all, 1.f / scale};
 
   const int packets = a.k / 8;
   for (int base = r0; base < r1; base += kRowThreads) {
@@ -1102,9 +1100,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
     slot[tid] = counts ? at : -1;
     if (counts) {
       float g = a.dloss[a.per_row ? row : 0];
-      if (a.mean) g /= static_cast<float>(all);
+      if (scaled) g = g / top * unit;
       if (target == -2) g = __int_as_float(0x7fc00000);  // a target outside the vocabulary poisons the gradients
-      g *= scale;
       a.row_index[at] = row;
       a.row_target[at] = target;
       a.row_lse[at] = a.lse[row];

@@ -301,7 +301,7 @@ class GradList:
 
 
 def _grad_list(grads, out=None) -> GradList:
-    if isinstance(grads, GradList):
+    if type(grads) is GradList:
         if out is not None:
             raise N.AxonError(N.AXON_E_ARG, "gradient list: a GradList has its own out")
         return grads
@@ -524,12 +524,17 @@ def silu_mlp(x, w1, w2, w3, *, out=None, out_dtype=None, workspace=None, tune=No
     return y
 
 
+_TARGET_BITS = {torch.int64: 64, torch.int32: 32}
 _REDUCE = {"none": N.AXON_REDUCE_NONE, "sum": N.AXON_REDUCE_SUM, "mean": N.AXON_REDUCE_MEAN}
 
 
-def _head_args(name, h, w, targets, reduction):
+def _head_args(name, h, w, targets, reduction, workspace):
     """Checks what the loss and its gradient share; (m, k, v, ld_h, ld_w, target bits, reduction)."""
-    _require_cuda(h, w, targets)
+    dev = h.device
+    if dev.type != "cuda" or w.device != dev or targets.device != dev or \
+            (workspace is not None and workspace.device != dev):
+        _require_cuda(h, w, targets, workspace)
+        raise N.AxonError(N.AXON_E_ARG, f"{name}: tensors on more than one device")
     m, k, ldh = _rows(h)
     v, kw, ldw = _rows(w)
     if kw != k:
@@ -538,17 +543,14 @@ def _head_args(name, h, w, targets, reduction):
         raise N.AxonError(N.AXON_E_UNSUPPORTED, f"{name}: h and w must share a type")
     if targets.shape != (m,) or not targets.is_contiguous():
         raise N.AxonError(N.AXON_E_SHAPE, f"{name}: targets must be contiguous [{m}]")
-    if targets.dtype not in (torch.int64, torch.int32):
+    bits = _TARGET_BITS.get(targets.dtype)
+    if bits is None:
         raise N.AxonError(N.AXON_E_UNSUPPORTED, f"{name}: targets must be int64 or int32")
-    if w.device != h.device or targets.device != h.device:
-        raise N.AxonError(N.AXON_E_ARG, f"{name}: tensors on more than one device")
-    if reduction not in _REDUCE:
+    red = _REDUCE.get(reduction)
+    if red is None:
         raise N.AxonError(N.AXON_E_ARG, f"{name}: reduction must be 'none', 'sum' or 'mean'")
-    if m <= 1:  # the stride of a single row says nothing
-        ldh = max(ldh, k)
-    if v == 1:
-        ldw = max(ldw, k)
-    return m, k, v, ldh, ldw, 8 * targets.element_size(), _REDUCE[reduction]
+    # the stride of a single row says nothing
+    return m, k, v, ldh if m > 1 else k, ldw if v > 1 else k, bits, red
 
 
 def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", workspace=None, tune=None):
@@ -560,17 +562,17 @@ def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", 
     [0, v) gives NaN. Returns (loss, stats): loss the per-row losses ("none"),
     their sum, or their mean over the rows not ignored, in fp32; stats [2, m]
     fp32 holds each row's log-sum-exp and loss, for linear_cross_entropy_grad."""
-    m, k, v, ldh, ldw, bits, red = _head_args("linear_cross_entropy", h, w, targets, reduction)
-    res = torch.empty(2 * m + 1, dtype=torch.float32, device=h.device)
-    stats, at = res.as_strided((2, m), (m, 1)), res.data_ptr()
-    loss = stats[1] if red == N.AXON_REDUCE_NONE else res[2 * m]
-    with _on_device(h.device):
-        need = _check_ws_bytes(N.lib().axon_linear_ce_workspace_bytes(m, k, v))
-        ws = _workspace(need, h.device, workspace)
-        check(N.lib().axon_linear_ce(_ptr(h), _ptr(w), _ptr(targets), at, at + 4 * m, at + 8 * m, m, k, v, ldh, ldw,
-                                     dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.numel(),
-                                     _tune(tune), _stream(h)))
-    return loss, stats
+    m, k, v, ldh, ldw, bits, red = _head_args("linear_cross_entropy", h, w, targets, reduction, workspace)
+    lib, dev = N.lib(), h.device
+    with _on_device(dev):
+        res = torch.empty(2 * m + 1, dtype=torch.float32, device=dev)
+        at = res.data_ptr()
+        ws = _workspace(_check_ws_bytes(lib.axon_linear_ce_workspace_bytes(m, k, v)), dev, workspace)
+        check(lib.axon_linear_ce(h.data_ptr(), w.data_ptr(), targets.data_ptr(), at, at + 4 * m, at + 8 * m, m, k, v,
+                                 ldh, ldw, dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.nbytes,
+                                 _tune(tune), _stream(h)))
+    stats = res.as_strided((2, m), (m, 1))
+    return stats[1] if red == N.AXON_REDUCE_NONE else res[2 * m], stats
 
 
 def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100, reduction="mean", need=(True, True),
@@ -584,33 +586,37 @@ def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100,
     tensors to write. Rows that are ignored get zeros. tune={"split": words}
     sets the piece of the vocabulary that is worked on at a time."""
     name = "linear_cross_entropy_grad"
-    m, k, v, ldh, ldw, bits, red = _head_args(name, h, w, targets, reduction)
-    _require_cuda(stats, dloss)
-    if stats.shape != (2, m) or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.device != h.device:
+    m, k, v, ldh, ldw, bits, red = _head_args(name, h, w, targets, reduction, workspace)
+    lib, dev = N.lib(), h.device
+    if stats.shape != (2, m) or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.device != dev:
         raise N.AxonError(N.AXON_E_ARG, f"{name}: stats must be the forward call's [2, {m}] fp32 tensor")
-    if dloss.dtype != torch.float32 or dloss.device != h.device or not dloss.is_contiguous() or \
+    if dloss.dtype != torch.float32 or dloss.device != dev or not dloss.is_contiguous() or \
             (dloss.shape != (m,) if red == N.AXON_REDUCE_NONE else dloss.numel() != 1):
         raise N.AxonError(N.AXON_E_ARG, f"{name}: dloss must be contiguous fp32, "
                           + (f"[{m}]" if red == N.AXON_REDUCE_NONE else "one value"))
+    lddh = lddw = k
     if out is not None:
         dh, dw = out
-    else:
-        dh = torch.empty((m, k), dtype=h.dtype, device=h.device) if need[0] else None
-        dw = torch.empty((v, k), dtype=dw_dtype or w.dtype, device=h.device) if need[1] else None
-    _require_cuda(dh, dw)
-    for t, like, types in ((dh, h, (h.dtype,)), (dw, w, (w.dtype, torch.float32))):
-        if t is not None and (t.shape != like.shape or t.dtype not in types or t.device != h.device):
-            raise N.AxonError(N.AXON_E_ARG, f"{name}: out must have the operands' shapes and types")
-    lddh = max(_rows(dh)[2], k) if dh is not None else 0
-    lddw = max(_rows(dw)[2], k) if dw is not None else 0
-    with _on_device(h.device):
-        nbytes = _check_ws_bytes(N.lib().axon_linear_ce_grad_workspace_bytes(m, k, v, _tune(tune)))
-        ws = _workspace(nbytes, h.device, workspace)
-        check(N.lib().axon_linear_ce_grad(_ptr(h), _ptr(w), _ptr(targets), stats.data_ptr(),
-                                          stats.data_ptr() + 4 * m, _ptr(dloss), _ptr(dh), _ptr(dw), m, k, v, ldh,
-                                          ldw, lddh, lddw, dtype_code(h), dtype_code(dw) if dw is not None else
-                                          dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.numel(),
-                                          _tune(tune), _stream(h)))
+        for t, like, types in ((dh, h, (h.dtype,)), (dw, w, (w.dtype, torch.float32))):
+            if t is not None and (t.shape != like.shape or t.dtype not in types or t.device != dev):
+                raise N.AxonError(N.AXON_E_ARG, f"{name}: out must have the operands' shapes and types")
+        if dh is not None and m > 1:
+            lddh = _rows(dh)[2]
+        if dw is not None and v > 1:
+            lddw = _rows(dw)[2]
+    elif dw_dtype not in (None, w.dtype, torch.float32):
+        raise N.AxonError(N.AXON_E_ARG, f"{name}: dw has w's type or fp32")
+    with _on_device(dev):
+        if out is None:
+            dh = torch.empty((m, k), dtype=h.dtype, device=dev) if need[0] else None
+            dw = torch.empty((v, k), dtype=dw_dtype or w.dtype, device=dev) if need[1] else None
+        tune_ref = _tune(tune)
+        ws = _workspace(_check_ws_bytes(lib.axon_linear_ce_grad_workspace_bytes(m, k, v, tune_ref)), dev, workspace)
+        at = stats.data_ptr()
+        check(lib.axon_linear_ce_grad(h.data_ptr(), w.data_ptr(), targets.data_ptr(), at, at + 4 * m, dloss.data_ptr(),
+                                      _ptr(dh), _ptr(dw), m, k, v, ldh, ldw, lddh, lddw, dtype_code(h),
+                                      dtype_code(h if dw is None else dw), bits, int(ignore_index), red, ws.data_ptr(),
+                                      ws.nbytes, tune_ref, _stream(h)))
     return dh, dw
 
 

@@ -438,6 +438,23 @@ def test_fp16_scales(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_common_weight_costs_no_digits(dtype, cuda_device):
+    """d is rounded before the loss's weight is applied, so the mean's gradient is
+    the sum's divided by the count up to fp32 roundings (three: the weight, and
+    a product each), whatever the count, and so is any power of the scale."""
+    h, w, t = _inputs(cuda_device, 77, 64, 900, dtype, seed=14, ignored=0.1)
+    count = int((t != IGNORE).sum())
+    one = torch.ones(1, device=cuda_device)
+    _, _, _, total = _both(h, w, t, one, "sum", dw_dtype=torch.float32)
+    _, _, _, mean = _both(h, w, t, one, "mean", dw_dtype=torch.float32)
+    assert bool(((mean.double() * count - total.double()).abs() <= 3 * U32 * total.double().abs()).all())
+    _, _, _, odd = _both(h, w, t, one * 0.3, "sum", dw_dtype=torch.float32)
+    third = float(torch.tensor(0.3))
+    assert bool(((odd.double() / third - total.double()).abs() <= 3 * U32 * total.double().abs()).all())
+
+
+@pytest.mark.gpu
 def test_wider_head(cuda_device):
     """Several tiles in every direction, more tiles than pairs, default piece
     and forced ones, bitwise repeatable."""
