@@ -62,14 +62,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode { kLse = 0, kDlogits = 1, kGrads = 2 };
 
-// Epilogue warps, and the 32 KB stages that fit the 227 KB. Two warps share a
-// TMEM lane quarter, half the columns each, where a tile is written: with few
-// k-blocks a tile the epilogue is the longest part. kLse has one per quarter, so
-// that a row's pair comes from one thread.
-constexpr int epi_warps(int mode) { return mode == kLse ? 4 : 8; }
+// Epilogue warps: two share a TMEM lane quarter, half the columns each. Stages:
+// as many of 32 KB as fit the 227 KB.
+constexpr int kEpiWarps = 8;
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;
 constexpr int stages_of(int mode) { return mode == kLse ? 7 : 6; }
-constexpr int pair_threads(int mode) { return 64 + 32 * epi_warps(mode); }
-constexpr int staging_of(int mode) { return mode == kLse ? 0 : epi_warps(mode) * kStaging; }
+constexpr int staging_of(int mode) { return mode == kLse ? 0 : kEpiWarps * kStaging; }
 constexpr int smem_of(int mode) { return stages_of(mode) * STAGE + staging_of(mode) + 1024 + 256; }
 
 // What ce_grad_rows hands to the kernels after it.
@@ -89,7 +87,7 @@ struct CeParams {
   int target64;
   int64_t ignore_index;
   float2* part;         // [m][parts]
-  int parts;            // word tiles (ce_pair) or CTAs (ce_narrow)
+  int parts;            // half word tiles (ce_pair) or CTAs (ce_narrow)
   unsigned* done;       // counts ce_stats' CTAs; set to 0 here
   // kDlogits: per counted row
   const int* row_target;
@@ -292,36 +290,72 @@ __device__ __forceinline__ float max32(const float* v) {
   return a[0];
 }
 
-// kLse: this thread's row over the tile's words.
-__device__ __forceinline__ void lse_tile(const CeParams& p, const Tile& t, uint32_t tbase, int64_t row, bool row_ok) {
+// This warp is done with the accumulator (its values are in registers).
+__device__ __forceinline__ void release_tmem(uint32_t leader_tempty, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_cluster(leader_tempty, 1);
+}
+
+// Waits for this thread's TMEM loads, and ties the 32 registers of one of them to
+// the wait, so that nothing reads them before it.
+__device__ __forceinline__ void tmem_wait_ld32(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+
+// 32 more words into a row's running maximum and sum; `left` of them count, and
+// the one at `target` (negative or past 31: none) does not.
+__device__ __forceinline__ void lse_words(float* v, int left, int target, float& mx, float& sum) {
   const float ninf = __int_as_float(0xff800000);
-  const int target = row_ok ? load_target(p.targets, p.target64, row, p.ignore_index, p.v) : -1;
-  float mx = ninf, sum = 0.f;
-#pragma unroll 1
-  for (int c = 0; c < p.word_tile; c += 32) {
-    const int col = t.tn * p.word_tile + c;
-    if (col >= p.v) break;  // the same for the whole warp
-    float v[32];
-    tmem_ld_cols<32>(tbase + c, v);
-    if (col + 32 > p.v) {
+  if (left < 32) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col + j >= p.v) v[j] = ninf;
-    }
-    if (target >= col && target < col + 32) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (target == col + j) v[j] = ninf;
-    }
-    const float nm = fmaxf(mx, max32(v));
-    const float ref = nm == ninf ? 0.f : nm;  // nothing counted yet: exp gives 0
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 32; ++j) s[j & 3] += exp_from(v[j], ref);
-    sum = sum * exp_from(mx, ref) + ((s[0] + s[1]) + (s[2] + s[3]));
-    mx = nm;
+    for (int j = 0; j < 32; ++j)
+      if (j >= left) v[j] = ninf;
   }
-  if (row_ok) p.part[row * p.parts + t.tn] = make_float2(mx, sum);
+  if (target >= 0 && target < 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (target == j) v[j] = ninf;
+  }
+  const float nm = fmaxf(mx, max32(v));
+  const float ref = nm == ninf ? 0.f : nm;  // nothing counted yet: exp gives 0
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[j & 3] += exp_from(v[j], ref);
+  sum = sum * exp_from(mx, ref) + ((s[0] + s[1]) + (s[2] + s[3]));
+  mx = nm;
+}
+
+// kLse: this thread's row over half of the tile's words, the next 32 on their way
+// from tensor memory (a load takes some 450 cycles) while 32 are worked on.
+__device__ __forceinline__ void lse_tile(const CeParams& p, const Tile& t, uint32_t tbase, int half, int64_t row,
+                                         bool row_ok, int target, int lane, uint32_t tempty) {
+  const int words = p.word_tile / 2, at = half * words, col = t.tn * p.word_tile + at;
+  const int count = min(words, p.v - col);  // the same for the whole warp; may be negative
+  target -= col;
+  float mx = __int_as_float(0xff800000), sum = 0.f;
+  float a[32], b[32];
+  __syncwarp();
+  if (count > 0) tmem_ld32(tbase + at, a);
+#pragma unroll 1
+  for (int c = 0; c < count; c += 64) {
+    tmem_wait_ld32(a);
+    if (c + 32 < count) tmem_ld32(tbase + at + c + 32, b);
+    lse_words(a, count - c, target - c, mx, sum);
+    if (c + 32 >= count) break;
+    tmem_wait_ld32(b);
+    if (c + 64 < count) tmem_ld32(tbase + at + c + 64, a);
+    lse_words(b, count - c - 32, target - c - 32, mx, sum);
+  }
+  release_tmem(tempty, lane);
+  if (row_ok) p.part[row * p.parts + t.tn * 2 + half] = make_float2(mx, sum);
 }
 
 // A thread holds a row of an accumulator tile, so its stores would touch 32 rows
@@ -356,13 +390,6 @@ __device__ __forceinline__ void store_staged(const CUtensorMap* map, uint8_t* st
 __device__ __forceinline__ void staging_free(int lane) {
   if (lane == 0) tma_store_wait_read();
   __syncwarp();
-}
-
-// This warp is done with the accumulator (its values are in registers).
-__device__ __forceinline__ void release_tmem(uint32_t leader_tempty, int lane) {
-  tc_fence_before();
-  __syncwarp();
-  if (lane == 0) mbar_arrive_cluster(leader_tempty, 1);
 }
 
 // Rows of d that the contraction over rows reads: the counted ones up to the
@@ -494,7 +521,7 @@ __device__ __forceinline__ void dh_tile(const CeParams& p, const Tile& t, uint32
 // ---- the CTA-pair kernel ---------------------------------------------------------------
 
 template <int MODE, typename T, typename TW>
-__global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_constant__ CeParams p) {
+__global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant__ CeParams p) {
   constexpr int kStages = stages_of(MODE);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -520,7 +547,7 @@ __global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_co
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 2 * epi_warps(MODE));  // one arrival per epilogue warp of each CTA
+      mbar_init(&tempty[b], 2 * kEpiWarps);  // one arrival per epilogue warp of each CTA
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -613,17 +640,20 @@ __global__ void __launch_bounds__(pair_threads(MODE), 1) ce_pair(const __grid_co
     const float unscale = MODE == kGrads ? p.header->unscale : 1.f;
     for (int i = 0; w.at(p, i, t); ++i) {
       const int buf = i & 1;
+      const int64_t row0 = static_cast<int64_t>(t.tm) * 2 * BM + rank * BM + q * 32;  // of this warp's 32
+      const bool row_ok = row0 + lane < w.rows;
+      int target = -1;
+      if (MODE == kLse && row_ok)  // on its way while the tile is computed
+        target = load_target(p.targets, p.target64, row0 + lane, p.ignore_index, p.v);
       if (!mbar_wait(&tfull[buf], (i >> 1) & 1, abort_flag, &g_ce_error)) break;
       tc_fence_after();
-      const int64_t row0 = static_cast<int64_t>(t.tm) * 2 * BM + rank * BM + q * 32;  // of this warp's 32
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * BN);
       const uint32_t leader_tempty = mapa_u32(smem_u32(&tempty[buf]), 0);
+      const int half = warp < 6 ? 0 : 1, c0 = half * (BN / 2);  // this warp's half of the columns
       if constexpr (MODE == kLse) {
-        lse_tile(p, t, tbase, row0 + lane, row0 + lane < w.rows);
-        release_tmem(leader_tempty, lane);
+        lse_tile(p, t, tbase, half, row0 + lane, row_ok, target, lane, leader_tempty);
       } else {
         uint8_t* stg = staging + (warp - 2) * kStaging;
-        const int half = warp < 6 ? 0 : 1, c0 = half * (BN / 2);  // this warp's half of the columns
         if constexpr (MODE == kDlogits) dlogits_tile<T>(p, t, tbase, half, row0, lane, w.rows, stg, leader_tempty);
         else if (t.dw) dw_tile<TW>(p, t, tbase, c0, row0, lane, unscale, stg, leader_tempty);
         else dh_tile<T>(p, t, tbase, c0, row0, lane, w.rows, unscale, stg, leader_tempty);
@@ -1197,7 +1227,7 @@ int launch_pair(const char* what, const CeParams& p, int64_t tiles, int max_ctas
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.blockDim = dim3(pair_threads(MODE), 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = smem_of(MODE);
   cfg.stream = s;
   cfg.attrs = attr;
@@ -1318,12 +1348,13 @@ int grad_plan(int64_t m, int64_t k, int64_t v, const axon_tune_t& t, GradPlan& g
   // A dh tile contracts over the whole piece while a dw tile contracts over the
   // rows: with few rows, few pairs would work on dh long after the rest. Cut
   // the contraction so that a part is at most a third of a pair's share, down
-  // to 16 k-blocks. (64 x 2048 x 32000: 174 us uncut; 1001 x 1024 x 50257: 286.)
+  // to 16 k-blocks and to what a dw tile takes. (64 x 2048 x 32000: 174 us uncut; 1001 x 1024 x 50257: 286.)
   const int64_t cols = (k + BN - 1) / BN, kb_dh = (g.piece + BK - 1) / BK, kb_dw = (m + BK - 1) / BK;
   const int64_t n_dh = (m + 255) / 256 * cols, n_dw = g.piece / 256 * cols;
   const int64_t pairs = sm_count() / 2;
   const int64_t share = (n_dh * (kb_dh + kTileCost) + n_dw * (kb_dw + kTileCost)) / pairs;
   int64_t part = share / 3 > 16 ? share / 3 : 16;
+  if (part < kb_dw) part = kb_dw;
   if (part > kb_dh) part = kb_dh;
   g.splits = static_cast<int>((kb_dh + part - 1) / part);
   g.off_rows = 256;
@@ -1452,7 +1483,7 @@ int64_t axon_linear_ce_workspace_bytes(int64_t m, int64_t k, int64_t v) {
   int rc = check_sizes("axon_linear_ce", m, k, v);
   if (rc) return rc;
   const int64_t words = wide_words(m, v);
-  return 256 + round_up(m * (m > kNarrowRows ? (v + words - 1) / words : sm_count()) * 8, 256);
+  return 256 + round_up(m * (m > kNarrowRows ? (v + words - 1) / words * 2 : sm_count()) * 8, 256);
 }
 
 int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse, float* loss_rows, float* loss,
@@ -1485,7 +1516,7 @@ int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse
   p.done = static_cast<unsigned*>(workspace);
   p.part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 256);
   p.word_tile = logits_words(m, v, t.max_ctas);
-  p.parts = static_cast<int>(m > kNarrowRows ? (v + p.word_tile - 1) / p.word_tile : narrow_grid(v, t.max_ctas));
+  p.parts = static_cast<int>(m > kNarrowRows ? (v + p.word_tile - 1) / p.word_tile * 2 : narrow_grid(v, t.max_ctas));
   p.band = band_of(k);
   if ((rc = logits_maps(what, p, h, ld_h, w, ld_w, dtype))) return rc;
   const StatsArgs a{h, w, ld_h, ld_w, p.part, targets, p.target64, ignore_index, p.m, p.k, p.v, p.parts, lse, loss_rows,

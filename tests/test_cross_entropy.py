@@ -117,10 +117,10 @@ def test_variants_are_listed():
 
 
 def test_workspaces():
-    """The loss needs 8 bytes per row and 256 words; the gradient holds d by
+    """The loss needs 16 bytes per row and 256 words; the gradient holds d by
     pieces of at most 512 MB, and an fp32 dh only where there are several."""
     lib = N.lib()
-    assert lib.axon_linear_ce_workspace_bytes(4096, 4096, 128256) < 4096 * 501 * 8 + 4096 * 4 + 1024
+    assert lib.axon_linear_ce_workspace_bytes(4096, 4096, 128256) < 4096 * 501 * 16 + 4096 * 4 + 1024
     assert lib.axon_linear_ce_workspace_bytes(4, 60, 100) == N.AXON_E_SHAPE
     one = lib.axon_linear_ce_grad_workspace_bytes(256, 64, 1000, None)
     assert one < 256 * 1024 * 2 + 256 * 64 * 2 + 256 * 20 + 2048
