@@ -125,6 +125,12 @@ __device__ __forceinline__ float ex2(float x) {
 // exp(x - ref)
 __device__ __forceinline__ float exp_from(float x, float ref) { return ex2((x - ref) * kLog2e); }
 
+// mbar_wait by a whole warp, with one answer for all its lanes: where a wait
+// gives up, no lane goes on to the warp-wide instructions behind it alone.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_ce_error));
+}
+
 // ---- tiles -----------------------------------------------------------------------------
 
 struct Tile {
@@ -645,7 +651,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant
       int target = -1;
       if (MODE == kLse && row_ok)  // on its way while the tile is computed
         target = load_target(p.targets, p.target64, row0 + lane, p.ignore_index, p.v);
-      if (!mbar_wait(&tfull[buf], (i >> 1) & 1, abort_flag, &g_ce_error)) break;
+      if (!warp_wait(&tfull[buf], (i >> 1) & 1, abort_flag)) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * BN);
       const uint32_t leader_tempty = mapa_u32(smem_u32(&tempty[buf]), 0);
@@ -863,7 +869,7 @@ __global__ void __launch_bounds__(narrow_threads(NT), 1) ce_narrow(const __grid_
     int i = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
       const int buf = i & 1;
-      if (!mbar_wait(&tfull[buf], (i >> 1) & 1, abort_flag, &g_ce_error)) break;
+      if (!warp_wait(&tfull[buf], (i >> 1) & 1, abort_flag)) break;
       tc_fence_after();
       // lanes past the tile's words hold what the stage held before
       const int word = q * 32 + lane < p.word_tile ? t * p.word_tile + q * 32 + lane : 0x7fffffff;

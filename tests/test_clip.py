@@ -195,6 +195,37 @@ def test_same_bits_every_time_and_large_list(cuda_device):
 
 
 @pytest.mark.gpu
+def test_a_tensor_past_32_bits(cuda_device):
+    """2^31 + 4099 elements: every one counts, every one is scaled."""
+    n = 2 ** 31 + 4099
+    x = torch.full((n,), 0.5, dtype=torch.bfloat16, device=cuda_device)
+    x[-1] = 2.0
+    want = (0.25 * (n - 1) + 4.0) ** 0.5
+    out, norm = ops.clip_grads([x], want / 4)
+    assert abs(float(norm) - want) <= NORM_TOL * want
+    assert float(out[0][-1]) == 0.5
+    head, tail = out[0][:2 ** 30], out[0][2 ** 30:-1]
+    assert bool((head == 0.125).all()) and bool((tail == 0.125).all())
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(cuda_device):
+    """Calls in flight on two streams share nothing."""
+    a = _make(cuda_device, [(3001, 77)] * 30, DTYPES, seed=1)
+    b = _make(cuda_device, [(999,)] * 5, DTYPES, seed=2)
+    want = [ops.grad_norm(a), ops.grad_norm(b)]
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for s, g in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(ops.grad_norm(g))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i % 2]) for i, x in enumerate(got))
+
+
+@pytest.mark.gpu
 def test_nonfinite_and_zero(cuda_device):
     z = [torch.zeros(100, device=cuda_device)]
     norm, scale = ops.grad_norm_scale(z, 1.0)

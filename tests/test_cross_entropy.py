@@ -269,6 +269,36 @@ def test_gradients(shape, dtype, reduction, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,split", [((5, 64, 4160), 4096), ((130, 520, 9000), 8192), ((40, 64, 12345), 0)])
+def test_pieces_whose_contraction_is_cut(shape, split, cuda_device):
+    """dh's contraction over a piece in parts, the last piece shorter than the
+    others (some of its parts empty)."""
+    m, k, v = shape
+    lib = N.lib()
+    tune = {"split": split}
+    whole = split or -(-v // 256) * 256
+    assert lib.axon_linear_ce_grad_workspace_bytes(m, k, v, N.Tune.of(tune)) > \
+        256 + 5 * m * 4 + m * k * 2 + m * whole * 2 + 2 * m * k * 4  # several fp32 parts of dh
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=v, ignored=0.2)
+    dloss = torch.ones(1, device=cuda_device)
+    _, _, dh, dw = _both(h, w, t, dloss, "sum", tune=tune)
+    Ref(h, w, t, _row_g(dloss, t, "sum")).check_grads(dh, dw)
+
+
+@pytest.mark.gpu
+def test_bands_of_rows(cuda_device):
+    """A hidden size whose rows of h fill L2's share in a few row tiles, so the
+    logits are walked in several bands."""
+    m, k, v = 1300, 24584, 700
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=3, ignored=0.1)
+    dloss = torch.ones(1, device=cuda_device)
+    _, stats, dh, dw = _both(h, w, t, dloss, "mean")
+    ref = Ref(h, w, t, _row_g(dloss, t, "mean"))
+    ref.check_loss(stats)
+    ref.check_grads(dh, dw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("split", [256, 512, 1024])
 @pytest.mark.parametrize("shape", [(5, 64, 1000), (300, 264, 2049), (513, 512, 1281)])
 def test_pieces_of_the_vocabulary(shape, split, cuda_device):
@@ -502,6 +532,61 @@ def test_other_stream_and_graph(cuda_device):
         want = _both(h, w, t, dloss, "mean")
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(cuda_device):
+    """Calls in flight on two streams share nothing."""
+    h, w, t = _inputs(cuda_device, 300, 128, 3000, torch.bfloat16, seed=51, ignored=0.2)
+    dloss = torch.ones(1, device=cuda_device)
+    wants = [_both(h[:n], w, t[:n], dloss, "mean") for n in (300, 40)]
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s, n in zip(streams, (300, 40)):
+            with torch.cuda.stream(s):
+                loss, stats = ops.linear_cross_entropy(h[:n], w, t[:n])
+                got.append((loss, stats, *ops.linear_cross_entropy_grad(h[:n], w, t[:n], stats, dloss)))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for a, b in zip(g, wants[i % 2]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda_device):
+    """A head of 2.3e9 entries (offsets past 2^31 elements and 2^32 bytes), with
+    few rows and with a row tile; the loss in full, dw in its first and last
+    words, dh of one row."""
+    k, v = 8192, 280001
+    h, w, t = _inputs(cuda_device, 200, k, v, torch.bfloat16, seed=61)
+    t[0] = v - 1
+    for m in (3, 200):
+        dloss = torch.ones(1, device=cuda_device)
+        _, stats, dh, dw = _both(h[:m], w, t[:m], dloss, "sum")
+        hd = h[:m].double()
+        rows = torch.arange(m, device=cuda_device)
+        s = torch.cat([hd @ w[i:i + 20000].double().T for i in range(0, v, 20000)], dim=1)
+        st = s[rows, t[:m]].clone()
+        s[rows, t[:m]] = -math.inf
+        rest = torch.logsumexp(s, dim=1)
+        loss = torch.logaddexp(rest - st, torch.zeros_like(rest))
+        a = float((hd.abs().sum(dim=1) * w.abs().max().double()).max())  # at least sum |h w|
+        ds = (k / 16 + 4) * 2.0 ** -23 * a
+        assert bool(((stats[1].double() - loss).abs() <= loss.clamp(max=1.0) * (2 * ds + E) + U32 * loss).all())
+        d = torch.exp(s - (rest + torch.log1p(torch.exp(st - rest)))[:, None])
+        d[rows, t[:m]] = torch.expm1(-loss)
+        r = 2 * ds + 2 * E + 2.0 ** -8
+        for at in (slice(0, 500), slice(v - 500, v)):
+            want, size = d[:, at].T @ hd, d[:, at].abs().T @ hd.abs()
+            tol = (r + (m / 16 + 4) * 2.0 ** -23) * size + 2.0 ** -8 * want.abs()
+            assert bool(((dw[at].double() - want).abs() <= tol).all())
+        want = sum(d[:1, i:i + 20000] @ w[i:i + 20000].double() for i in range(0, v, 20000))
+        size = sum(d[:1, i:i + 20000].abs() @ w[i:i + 20000].double().abs() for i in range(0, v, 20000))
+        tol = (r + (v / 16 + 68) * 2.0 ** -23) * size + 2.0 ** -8 * want.abs()
+        assert bool(((dh[:1].double() - want).abs() <= tol).all())
+        del s, d, dw
 
 
 @pytest.mark.gpu
