@@ -158,8 +158,8 @@ constexpr int kFewRows = 8;
 // fastest for dh and column tiles for dw, so that the pairs share the words,
 // and d, in L2. With few rows, even pairs begin with dh and odd ones with dw: dh is
 // then bound by reading w and dw by writing, and memory that only writes moves
-// 3.9 TB/s here, against 6.6 both ways (gradients of 64 x 2048 x 32000: 120 us,
-// all pairs beginning with dh 127; with 4096 rows it costs 4%).
+// 3.9 TB/s here, against 6.6 both ways (6% off the gradients of 64 x 2048 x 32000;
+// with 4096 rows it would cost 4%).
 template <int MODE>
 struct Walk {
   int pair, pairs, rows;
@@ -525,6 +525,12 @@ __device__ __forceinline__ void dh_tile(const CeParams& p, const Tile& t, uint32
 }
 
 // ---- the CTA-pair kernel ---------------------------------------------------------------
+//
+// Bound by the tensor pipe from some 300 rows up: it is 86-87% active in all three
+// modes at 2048 x 4096 x 65536, where the loss runs 1551 TFLOP/s, d 1516 and the
+// products 1484 in a burst (cuBLAS here: 1583). At hidden sizes of 512 and less the
+// epilogue shows: 3.1 us a tile at k = 64 (reading 128 KB of tensor memory, the
+// exponentials, and the tile's latencies), against 2.2 us of MMA at k = 512.
 
 template <int MODE, typename T, typename TW>
 __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant__ CeParams p) {
@@ -696,6 +702,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant
 //             lanes are joined once, at the end, into one (max, sum) per row
 //             and CTA;
 //   kDlogits  a warp's 32 lanes are 32 neighbouring words of a row of d.
+//
+// One row against 128256 words of 4096: 165 us, 6.4 TB/s (0.97 of a copy's rate;
+// the 256-row tiles took 256). 64 rows x 2048 x 32000: 27 us, 4.9 TB/s. 128 rows x
+// 4096 x 128256: 190 us (212).
 constexpr int kNarrowRows = 128;
 constexpr int kNarrowMaxStages = 12;
 
@@ -992,7 +1002,8 @@ struct StatsArgs {
 constexpr int kStatsThreads = 128;
 constexpr int kStatsRows = kStatsThreads / 32;
 
-// Joins a row's (max, sum) parts with the target's logit, a warp per row; the
+// Joins a row's (max, sum) parts with the target's logit, a warp per row (27 us
+// for 4096 rows of k = 4096, most of it the targets' rows of w); the
 // CTA that comes last adds the rows' losses up, in row order whichever CTA it
 // is.
 template <typename T>
@@ -1087,8 +1098,9 @@ constexpr int kRowThreads = 256;
 
 // Moves the rows that count to the front. Every CTA owns a range of rows; it
 // finds the number of counted rows before its own, and the largest |g|, by
-// reading all targets itself: m is at most some ten thousands, and a
-// second launch would cost more.
+// reading all targets itself: m is at most some ten thousands, and a second
+// launch would cost more. Bound by the copy of h: 18 us at 4096 x 4096, 6 at 64
+// rows.
 __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
   __shared__ int slot[kRowThreads];
   __shared__ int warp_count[kRowThreads / 32];
@@ -1167,7 +1179,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
 }
 
 // dh = unscale * sum over the splits for the counted rows. Four lanes share 8
-// columns, each adding every fourth split in order, and are joined in order.
+// columns, each adding every fourth split in order, and are joined in order. 5-8
+// us where dh is cut at all.
 template <typename T>
 __global__ void __launch_bounds__(256) ce_dh_finish(const float* __restrict__ acc, const RowHeader* header,
                                                     const int* __restrict__ row_index, int m, int k, int splits, T* dh,
@@ -1354,7 +1367,8 @@ int grad_plan(int64_t m, int64_t k, int64_t v, const axon_tune_t& t, GradPlan& g
   // A dh tile contracts over the whole piece while a dw tile contracts over the
   // rows: with few rows, few pairs would work on dh long after the rest. Cut
   // the contraction so that a part is at most a third of a pair's share, down
-  // to 16 k-blocks and to what a dw tile takes. (64 x 2048 x 32000: 174 us uncut; 1001 x 1024 x 50257: 286.)
+  // to 16 k-blocks and to what a dw tile takes. Uncut, the products of 64 x 2048
+  // x 32000 took 174 us (103 cut, all else equal), of 1001 x 1024 x 50257 286 (170).
   const int64_t cols = (k + BN - 1) / BN, kb_dh = (g.piece + BK - 1) / BK, kb_dw = (m + BK - 1) / BK;
   const int64_t n_dh = (m + 255) / 256 * cols, n_dw = g.piece / 256 * cols;
   const int64_t pairs = sm_count() / 2;
