@@ -28,6 +28,9 @@
 //             until the last piece) and tiles of dw (d transposed, taken by TMA as
 //             an MN-major A operand, contracted over the rows).
 //
+// Up to 128 rows, where memory is the bound, ce_narrow takes the place of the
+// first two and ce_few of the third.
+//
 // The gradient works on the rows that count: ce_grad_rows moves them to the
 // front (a copy of h, a few microseconds) and hands the later kernels their
 // number on the device, so ignored rows cost nothing and whatever they hold
@@ -77,7 +80,7 @@ struct RowHeader {
 };
 
 struct CeParams {
-  CUtensorMap a, b;     // kLse, kDlogits: h, w.   kGrads, dh tiles: d, w's piece
+  CUtensorMap a, b;     // kLse, kDlogits: h, w.   kGrads and ce_few, dh tiles: d, w's piece
   CUtensorMap a2, b2;   // kGrads, dw tiles: d transposed, h
   CUtensorMap c;        // what the epilogue writes by TMA: kDlogits d, kGrads dw
   int m, v, k;          // rows (at most), words of this piece, hidden size
@@ -105,6 +108,7 @@ struct CeParams {
   float* acc;           // fp32 [splits][m][k]: dh between pieces, and its splits
   int first, last;      // this piece is the vocabulary's first / last
   int splits;           // parts that dh's contraction over the piece is cut into
+  int few;              // ce_few's rows of a dh tile (32, 64 or 128), 0: ce_pair
   int word_tile;        // kLse, kDlogits: words a tile
   int band;             // row tiles of s visited together
 };
@@ -158,8 +162,8 @@ constexpr int kFewRows = 8;
 // fastest for dh and column tiles for dw, so that the pairs share the words,
 // and d, in L2. With few rows, even pairs begin with dh and odd ones with dw: dh is
 // then bound by reading w and dw by writing, and memory that only writes moves
-// 3.9 TB/s here, against 6.6 both ways (6% off the gradients of 64 x 2048 x 32000;
-// with 4096 rows it would cost 4%).
+// 3.9 TB/s here, against 6.6 both ways (6% off the gradients of 64 x 2048 x 32000
+// when they ran here; with 4096 rows it would cost 4%).
 template <int MODE>
 struct Walk {
   int pair, pairs, rows;
@@ -265,13 +269,13 @@ __device__ __forceinline__ void load_stage(const CeParams& p, const Tile& t, int
   }
 }
 
-// tcgen05 instruction descriptor: fp32 accumulator, M 256, N columns; bit 15 / 16:
+// tcgen05 instruction descriptor: fp32 accumulator, M rows (256 a pair), N columns; bit 15 / 16:
 // A / B is MN-major.
 template <typename T>
-__device__ __forceinline__ uint32_t idesc(int n, bool a_mn, bool b_mn) {
+__device__ __forceinline__ uint32_t idesc(int n, bool a_mn, bool b_mn, int m = 2 * BM) {
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>((2 * BM) >> 4) << 24);
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 // ---- epilogues -----------------------------------------------------------------------
@@ -392,9 +396,11 @@ __device__ __forceinline__ void store_staged(const CUtensorMap* map, uint8_t* st
   if (lane == 0) tma_store_2d(map, stg, col, row);
 }
 
-// Before the staging memory is written again.
+// Before the staging memory is written again: all but the last LEFT stores have
+// read theirs.
+template <int LEFT = 0>
 __device__ __forceinline__ void staging_free(int lane) {
-  if (lane == 0) tma_store_wait_read();
+  if (lane == 0) tma_store_wait_read<LEFT>();
   __syncwarp();
 }
 
@@ -454,26 +460,28 @@ __device__ __forceinline__ void store8(TO* dst, const float* v) {
   }
 }
 
-// kGrads, columns [c0, c0 + 128) of a tile of dw, rounded (row0 the warp's first
+// Columns [c0, c0 + 128) of a tile of dw, rounded (row0 the warp's first
 // word within the piece). The accumulator is released once its last part is in
-// registers: with few rows a tile is one or two k-blocks, and the pair would
-// wait for its epilogue.
-template <typename TW>
-__device__ __forceinline__ void dw_tile(const CeParams& p, const Tile& t, uint32_t tbase, int c0, int64_t row0,
-                                        int lane, float unscale, uint8_t* stg, uint32_t tempty) {
+// registers: with few rows a tile is one or two k-blocks, and its MMA would wait
+// for the epilogue. BUFS staging buffers are used in turn.
+template <typename TW, int BUFS>
+__device__ __forceinline__ void dw_tile(const CeParams& p, int tn, int kb, uint32_t tbase, int c0, int64_t row0,
+                                        int lane, float unscale, uint8_t* staging, uint32_t& turn, uint32_t tempty) {
   constexpr int COLS = 128 / sizeof(TW);
 #pragma unroll 1
   for (int c = 0; c < BN / 2; c += COLS) {
-    const int col = t.tn * BN + c0 + c;
+    const int col = tn * BN + c0 + c;
     float v[COLS];
     tmem_ld_cols<COLS>(tbase + c0 + c, v);
     if (c + COLS == BN / 2) release_tmem(tempty, lane);
     if (row0 >= p.v || col >= p.k) continue;  // the same for the whole warp
 #pragma unroll
-    for (int j = 0; j < COLS; ++j) v[j] = t.kb ? v[j] * unscale : 0.f;  // no k-block: nothing was accumulated
-    staging_free(lane);
+    for (int j = 0; j < COLS; ++j) v[j] = kb ? v[j] * unscale : 0.f;  // no k-block: nothing was accumulated
+    uint8_t* stg = staging + turn * kStaging;
+    staging_free<BUFS - 1>(lane);
     stage_row<TW>(stg, lane, v);
     store_staged(&p.c, stg, lane, col, static_cast<int>(row0));
+    if (BUFS > 1) turn ^= 1u;
   }
 }
 
@@ -650,6 +658,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant
     // ---------------- epilogue (both CTAs, their own 128 rows) ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
     const float unscale = MODE == kGrads ? p.header->unscale : 1.f;
+    uint32_t turn = 0;
     for (int i = 0; w.at(p, i, t); ++i) {
       const int buf = i & 1;
       const int64_t row0 = static_cast<int64_t>(t.tm) * 2 * BM + rank * BM + q * 32;  // of this warp's 32
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant
       } else {
         uint8_t* stg = staging + (warp - 2) * kStaging;
         if constexpr (MODE == kDlogits) dlogits_tile<T>(p, t, tbase, half, row0, lane, w.rows, stg, leader_tempty);
-        else if (t.dw) dw_tile<TW>(p, t, tbase, c0, row0, lane, unscale, stg, leader_tempty);
+        else if (t.dw) dw_tile<TW, 1>(p, t.tn, t.kb, tbase, c0, row0, lane, unscale, stg, turn, leader_tempty);
         else dh_tile<T>(p, t, tbase, c0, row0, lane, w.rows, unscale, stg, leader_tempty);
       }
     }
@@ -685,6 +694,302 @@ __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS)
                  : "memory");
+  }
+}
+
+// ---- few rows: both products, read and written at once ---------------------------------------
+//
+// Up to 128 rows the products are bound by memory: dh reads w, dw is written.
+// Memory that is only written moves 3.9 TB/s on this card and 6.6 both ways, so
+// the two run at the same time on every SM, as two pipelines of one CTA that
+// share nothing but the tensor pipe:
+//
+//   dh   transposed, 128 of its columns on the accumulator's lanes and the rows
+//        beside them (A: w's words x columns as they lie, MN-major; B: d). A
+//        k-block is 16 KB of w and 4-16 KB of d; two accumulators; warps 0
+//        (TMA), 1 (MMA) and 12-15 (a warp's 32 lanes are 32 neighbouring
+//        columns of a row).
+//   dw   128 words x 256 columns, one or two k-blocks of rows, so all epilogue: one
+//        accumulator, given back when its second half is in registers. A CTA
+//        keeps to one block of columns, so its part of h stays in shared memory,
+//        and neighbouring CTAs write neighbouring pieces of dw's rows. Warps 2
+//        (TMA), 3 (MMA) and 4-11, TMA stores.
+//
+// Gradients in all: 64 rows x 2048 x 32000 94 us (one after the other on CTA
+// pairs 105), one row x 4096 x 128256 591 us (620), where dw written alone takes
+// 3.3 TB/s of the 3.9 and dh alone reads w at 6.4.
+constexpr int kFewThreads = 512;
+constexpr int kFewDwStages = 2;                                 // of d transposed, 16 KB
+constexpr int few_h(int few) { return (few + BK - 1) / BK * 2 * B_BYTES; }  // h, 32 KB a k-block
+constexpr int few_bufs(int few) { return few > 64 ? 1 : 2; }    // staging buffers a warp
+constexpr int few_fixed(int few) {
+  return kFewDwStages * A_BYTES + few_h(few) + 8 * few_bufs(few) * kStaging + 1024 + 256;
+}
+constexpr int few_stage(int few) { return A_BYTES + few * BK * 2; }
+constexpr int few_stages(int few) { return (232448 - few_fixed(few)) / few_stage(few); }
+constexpr int few_smem(int few) { return few_stages(few) * few_stage(few) + few_fixed(few); }
+
+// 32 lanes x 16 consecutive 32-bit TMEM columns.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// A tile of dh, transposed: this thread's column (lane) of dh in every row.
+template <typename T>
+__device__ __forceinline__ void few_dh_tile(const CeParams& p, int split, int kb, uint32_t tbase, int64_t col, int lane,
+                                            int rows, float unscale, uint32_t tempty) {
+  const bool direct = p.last && p.splits == 1, ok = col < p.k;
+  float* acc = p.acc + static_cast<int64_t>(split) * p.m * p.k + col;
+#pragma unroll 1
+  for (int r = 0; r < rows; r += 16) {
+    float v[16];
+    __syncwarp();
+    tmem_ld16(tbase + r, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (!ok || r + j >= rows) continue;
+      float x = kb ? v[j] : 0.f;
+      float* at = acc + static_cast<int64_t>(r + j) * p.k;
+      if (!p.first) x += *at;
+      if (direct) static_cast<T*>(p.dh)[p.row_index[r + j] * p.ld_dh + col] = from_f<T>(x * unscale);
+      else *at = x;
+    }
+  }
+  release_tmem(tempty, lane);
+}
+
+template <int FEW, typename T, typename TW>
+__global__ void __launch_bounds__(kFewThreads, 1) ce_few(const __grid_constant__ CeParams p) {
+  constexpr int S = few_stages(FEW), SB = few_stage(FEW), BUFS = few_bufs(FEW);
+  static_assert(S >= 3, "w must be read ahead");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* dw_ring = smem + S * SB;
+  uint8_t* h_block = dw_ring + kFewDwStages * A_BYTES;
+  uint8_t* staging = h_block + few_h(FEW);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * BUFS * kStaging);  // dh
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* dw_full = tempty + 2;
+  uint64_t* dw_empty = dw_full + kFewDwStages;
+  uint64_t* dw_tfull = dw_empty + kFewDwStages;
+  uint64_t* dw_tempty = dw_tfull + 1;
+  uint64_t* h_full = dw_tempty + 1;
+  uint64_t* drain = h_full + 1;  // dh, dw
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* issued = reinterpret_cast<int*>(tmem_slot + 2);  // dh, dw
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 4);
+      mbar_init(&drain[b], 1);
+      issued[b] = 0;
+    }
+    for (int s = 0; s < kFewDwStages; ++s) {
+      mbar_init(&dw_full[s], 1);
+      mbar_init(&dw_empty[s], 1);
+    }
+    mbar_init(dw_tfull, 1);
+    mbar_init(dw_tempty, 8);
+    mbar_init(h_full, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  pdl_wait();
+  pdl_trigger();
+  const int rows = p.header->rows;
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t dw_tmem = tmem_base + BN;  // columns 256..511; dh's two accumulators are below
+
+  // dh: columns run fastest, so that neighbouring CTAs read neighbouring pieces of w's rows
+  const int dh_cols = (p.k + BM - 1) / BM;
+  const int n_dh = p.dh && rows > 0 ? dh_cols * p.splits : 0;
+  const int kb_all = (p.v + BK - 1) / BK, kb_dh = (kb_all + p.splits - 1) / p.splits;
+  const int dw_cols = (p.k + BN - 1) / BN;
+  const int kb_dw = (rows + BK - 1) / BK;
+  // dw: this CTA's block of columns, its first word tile and the step to the next
+  const int tn = blockIdx.x % dw_cols, step = gridDim.x / dw_cols;
+  const int tm0 = static_cast<int>(blockIdx.x) < step * dw_cols ? blockIdx.x / dw_cols : INT32_MAX;
+  const int word_tiles = p.dw ? (p.v + BM - 1) / BM : 0;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- dh: TMA ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x; t < n_dh; t += gridDim.x) {
+      const int split = t / dh_cols, col = (t - split * dh_cols) * BM;
+      const int k1 = min(kb_all, (split + 1) * kb_dh);
+      for (int kb = split * kb_dh; kb < k1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, &g_ce_error)) goto dh_loaded;
+        mbar_expect_tx(&full[stage], static_cast<uint32_t>(SB));
+        uint8_t* sa = smem + stage * SB;
+        tma_load_2d(&p.b, &full[stage], sa, col, kb * BK);
+        tma_load_2d(&p.b, &full[stage], sa + CHUNK, col + 64, kb * BK);
+        tma_load_2d(&p.a, &full[stage], sa + A_BYTES, kb * BK, 0);
+        issued[0] += 1;
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  dh_loaded:;
+  } else if (warp == 1 && lane == 0) {
+    // ---------------- dh: MMA ----------------
+    const uint32_t id = idesc<T>(FEW, true, false, BM);
+    int stage = 0, i = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x; t < n_dh; t += gridDim.x, ++i) {
+      const int buf = i & 1;
+      if (!mbar_wait(&tempty[buf], ((i >> 1) & 1) ^ 1u, abort_flag, &g_ce_error)) break;
+      tc_fence_after();
+      const uint32_t d = tmem_base + static_cast<uint32_t>(buf * FEW);
+      const int k0 = t / dh_cols * kb_dh, k1 = min(kb_all, k0 + kb_dh);
+      bool ok = true;
+      for (int kb = k0; kb < k1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, &g_ce_error)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + stage * SB);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          tc_mma(d, sdesc(sa + k * 2048, CHUNK, 1024), sdesc(sa + A_BYTES + k * 32, 16, 1024), id,
+                 ((kb - k0) | k) != 0);
+        tc_commit(&empty[stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      tc_commit(&tfull[buf]);
+    }
+    tc_commit(&drain[0]);  // TMEM is released only after every MMA has retired
+    volatile int never = 0;
+    mbar_wait(&drain[0], 0, &never, &g_ce_error);
+  } else if (warp == 2 && lane == 0) {
+    // ---------------- dw: TMA ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    if (tm0 < word_tiles && kb_dw > 0) {
+      mbar_expect_tx(h_full, static_cast<uint32_t>(kb_dw * 2 * B_BYTES));
+      for (int i = 0; i < kb_dw * (BN / 64); ++i)
+        tma_load_2d(&p.b2, h_full, h_block + i * CHUNK, tn * BN + i % (BN / 64) * 64, i / (BN / 64) * BK);
+      issued[1] += 1;
+    }
+    for (int tm = tm0; tm < word_tiles; tm += step) {
+      for (int kb = 0; kb < kb_dw; ++kb) {
+        if (!mbar_wait(&dw_empty[stage], phase ^ 1u, abort_flag, &g_ce_error)) goto dw_loaded;
+        mbar_expect_tx(&dw_full[stage], A_BYTES);
+        uint8_t* sa = dw_ring + stage * A_BYTES;
+        tma_load_2d(&p.a2, &dw_full[stage], sa, tm * BM, kb * BK);
+        tma_load_2d(&p.a2, &dw_full[stage], sa + CHUNK, tm * BM + 64, kb * BK);
+        if (++stage == kFewDwStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  dw_loaded:;
+  } else if (warp == 3 && lane == 0) {
+    // ---------------- dw: MMA ----------------
+    const uint32_t id = idesc<T>(BN, true, true, BM);
+    int stage = 0;
+    uint32_t phase = 0, use = 0;
+    for (int tm = tm0; tm < word_tiles; tm += step, use ^= 1u) {
+      if (!mbar_wait(dw_tempty, use ^ 1u, abort_flag, &g_ce_error)) break;
+      bool ok = kb_dw == 0 || tm != tm0 || mbar_wait(h_full, 0, abort_flag, &g_ce_error);
+      if (!ok) break;
+      tc_fence_after();
+      for (int kb = 0; kb < kb_dw; ++kb) {
+        if (!mbar_wait(&dw_full[stage], phase, abort_flag, &g_ce_error)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sa = smem_u32(dw_ring + stage * A_BYTES), sb = smem_u32(h_block + kb * 2 * B_BYTES);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          tc_mma(dw_tmem, sdesc(sa + k * 2048, CHUNK, 1024), sdesc(sb + k * 2048, CHUNK, 1024), id, (kb | k) != 0);
+        tc_commit(&dw_empty[stage]);
+        if (++stage == kFewDwStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      tc_commit(dw_tfull);
+    }
+    tc_commit(&drain[1]);
+    volatile int never = 0;
+    mbar_wait(&drain[1], 0, &never, &g_ce_error);
+  } else if (warp >= 12) {
+    // ---------------- dh: epilogue ----------------
+    const int q = warp & 3;  // TMEM lane quarter this warp may access
+    const float unscale = p.header->unscale;
+    int i = 0;
+    for (int t = blockIdx.x; t < n_dh; t += gridDim.x, ++i) {
+      const int buf = i & 1;
+      if (!warp_wait(&tfull[buf], (i >> 1) & 1, abort_flag)) break;
+      tc_fence_after();
+      const int split = t / dh_cols, kb = min(kb_all, (split + 1) * kb_dh) - split * kb_dh;
+      const int64_t col = static_cast<int64_t>(t - split * dh_cols) * BM + q * 32 + lane;
+      few_dh_tile<T>(p, split, kb > 0 ? kb : 0, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * FEW, col,
+                     lane, rows, unscale, mapa_u32(smem_u32(&tempty[buf]), 0));
+    }
+  } else if (warp >= 4) {
+    // ---------------- dw: epilogue ----------------
+    const int q = warp & 3, c0 = warp < 8 ? 0 : BN / 2;
+    const float unscale = p.header->unscale;
+    uint8_t* stg = staging + (warp - 4) * BUFS * kStaging;
+    uint32_t use = 0, turn = 0;
+    for (int tm = tm0; tm < word_tiles; tm += step, use ^= 1u) {
+      if (!warp_wait(dw_tfull, use, abort_flag)) break;
+      tc_fence_after();
+      dw_tile<TW, BUFS>(p, tn, kb_dw, dw_tmem + (static_cast<uint32_t>(q * 32) << 16), c0,
+                        static_cast<int64_t>(tm) * BM + q * 32, lane, unscale, stg, turn,
+                        mapa_u32(smem_u32(dw_tempty), 0));
+    }
+    if (lane == 0) tma_store_wait();
+  }
+
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && (issued[0] > 0 || issued[1] > 0)) {
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies issued may still be landing
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
   }
 }
 
@@ -722,19 +1027,6 @@ constexpr int narrow_smem(int mode, int nt) { return narrow_stages(mode, nt) * n
 constexpr int narrow_cols(int nt) { return nt < 32 ? nt : 32; }
 constexpr int narrow_epi_warps(int nt) { return 4 * nt / narrow_cols(nt); }
 constexpr int narrow_threads(int nt) { return 64 + 32 * narrow_epi_warps(nt); }
-
-// 32 lanes x 16 consecutive 32-bit TMEM columns.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // Joins (max, sum) pairs.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
@@ -1343,6 +1635,14 @@ int band_of(int64_t k) {
   return static_cast<int>(b < 1 ? 1 : b > 4096 ? 4096 : b);
 }
 
+// Rows of ce_few's dh tiles, or 0 where ce_pair works: more than 128 rows, or more
+// blocks of 256 columns than CTAs (each keeps to one).
+int few_rows(int64_t m, int64_t k, int max_ctas) {
+  const int64_t grid = max_ctas > 0 && max_ctas < sm_count() ? max_ctas : sm_count();
+  if (m > 128 || (k + BN - 1) / BN > grid) return 0;
+  return m <= 32 ? 32 : m <= 64 ? 64 : 128;
+}
+
 struct GradPlan {
   int64_t piece;     // words a piece
   int64_t pieces;
@@ -1351,6 +1651,15 @@ struct GradPlan {
 };
 
 constexpr int64_t kPieceBytes = 512ll << 20;  // of d
+
+int layout(int64_t m, int64_t k, GradPlan& g) {
+  g.off_rows = 256;
+  g.off_hc = g.off_rows + round_up(5 * m * 4, 256);
+  g.off_d = g.off_hc + round_up(m * k * 2, 256);
+  g.off_acc = g.off_d + round_up(m * g.piece * 2, 256);
+  g.bytes = g.off_acc + (g.pieces > 1 || g.splits > 1 ? round_up(g.splits * m * k * 4, 256) : 0);
+  return AXON_OK;
+}
 
 int grad_plan(int64_t m, int64_t k, int64_t v, const axon_tune_t& t, GradPlan& g) {
   if (t.split < 0 || t.split % 256) return fail(AXON_E_ARG, "axon_linear_ce_grad: split must be a multiple of 256 words");
@@ -1370,6 +1679,21 @@ int grad_plan(int64_t m, int64_t k, int64_t v, const axon_tune_t& t, GradPlan& g
   // to 16 k-blocks and to what a dw tile takes. Uncut, the products of 64 x 2048
   // x 32000 took 174 us (103 cut, all else equal), of 1001 x 1024 x 50257 286 (170).
   const int64_t cols = (k + BN - 1) / BN, kb_dh = (g.piece + BK - 1) / BK, kb_dw = (m + BK - 1) / BK;
+  if (few_rows(m, k, t.max_ctas)) {
+    // ce_few: the number of parts (of 8 k-blocks at least) that leaves the SMs
+    // the least uneven, among those that take each at most a few
+    const int64_t tiles = (k + BM - 1) / BM, sms = sm_count();
+    g.splits = 1;
+    double least = 1e30;
+    for (int64_t n = 1; n <= 3 * ((sms + tiles - 1) / tiles) && (n == 1 || kb_dh / n >= 8); ++n) {
+      const double time = static_cast<double>((tiles * n + sms - 1) / sms) / n;
+      if (time < least * 0.99) {
+        least = time;
+        g.splits = static_cast<int>(n);
+      }
+    }
+    return layout(m, k, g);
+  }
   const int64_t n_dh = (m + 255) / 256 * cols, n_dw = g.piece / 256 * cols;
   const int64_t pairs = sm_count() / 2;
   const int64_t share = (n_dh * (kb_dh + kTileCost) + n_dw * (kb_dw + kTileCost)) / pairs;
@@ -1377,12 +1701,7 @@ int grad_plan(int64_t m, int64_t k, int64_t v, const axon_tune_t& t, GradPlan& g
   if (part < kb_dw) part = kb_dw;
   if (part > kb_dh) part = kb_dh;
   g.splits = static_cast<int>((kb_dh + part - 1) / part);
-  g.off_rows = 256;
-  g.off_hc = g.off_rows + round_up(5 * m * 4, 256);
-  g.off_d = g.off_hc + round_up(m * k * 2, 256);
-  g.off_acc = g.off_d + round_up(m * g.piece * 2, 256);
-  g.bytes = g.off_acc + (g.pieces > 1 || g.splits > 1 ? round_up(g.splits * m * k * 4, 256) : 0);
-  return AXON_OK;
+  return layout(m, k, g);
 }
 
 int check_sizes(const char* what, int64_t m, int64_t k, int64_t v) {
@@ -1471,12 +1790,44 @@ int run_loss(const CeParams& p, const StatsArgs& a, int max_ctas, cudaStream_t s
   return launch_status(what);
 }
 
+template <int FEW, typename T, typename TW>
+int launch_few_rows(const char* what, const CeParams& p, int grid, cudaStream_t s) {
+  static bool set[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return fail(AXON_E_CUDA, "%s: no current device", what);
+  auto kern = ce_few<FEW, T, TW>;
+  if (!set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem(FEW));
+    if (e != cudaSuccess) return fail(AXON_E_LAUNCH, "%s: smem attribute: %s", what, cudaGetErrorString(e));
+    set[dev] = true;
+  }
+  cudaError_t e = launch_k(kern, dim3(grid), dim3(kFewThreads), few_smem(FEW), s, p);
+  if (e != cudaSuccess) return fail(AXON_E_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  return launch_status(what);
+}
+
+template <typename T, typename TW>
+int launch_few(const char* what, const CeParams& p, int grid, cudaStream_t s) {
+  switch (p.few) {
+    case 32: return launch_few_rows<32, T, TW>(what, p, grid, s);
+    case 64: return launch_few_rows<64, T, TW>(what, p, grid, s);
+    default: return launch_few_rows<128, T, TW>(what, p, grid, s);
+  }
+}
+
 // Both kernels of one piece.
 template <typename T>
 int run_piece(const CeParams& pl, const CeParams& pg, int32_t dw_dtype, int max_ctas, cudaStream_t s) {
   const char* what = "axon_linear_ce_grad";
   int rc = launch_logits<kDlogits, T>(what, pl, max_ctas, s);
   if (rc) return rc;
+  if (pg.few) {
+    int64_t grid = sm_count();
+    if (max_ctas > 0 && max_ctas < grid) grid = max_ctas;
+    return dw_dtype == AXON_F32 ? launch_few<T, float>(what, pg, static_cast<int>(grid), s)
+                                : launch_few<T, T>(what, pg, static_cast<int>(grid), s);
+  }
   const int64_t cols = (pg.k + BN - 1) / BN;
   const int64_t tiles = cols * ((pg.dh ? (pg.m + 255ll) / 256 * pg.splits : 0) + (pg.dw ? (pg.v + 255) / 256 : 0));
   if (dw_dtype == AXON_F32) return launch_pair<kGrads, T, float>(what, pg, tiles, max_ctas, s);
@@ -1645,7 +1996,8 @@ int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const
     CeParams pg = p;
     if ((rc = logits_maps(what, p, ra.hc, k, wp, ld_w, dtype))) return rc;
     if ((rc = make_map(&p.c, p.d, dtype, vc, m, p.ld_d, 64, 32, "d", what))) return rc;
-    if ((rc = make_map(&pg.a, p.d, dtype, vc, m, p.ld_d, BK, BM, "d", what))) return rc;
+    pg.few = few_rows(m, k, t.max_ctas);
+    if ((rc = make_map(&pg.a, p.d, dtype, vc, m, p.ld_d, BK, pg.few ? pg.few : BM, "d", what))) return rc;
     if ((rc = make_map(&pg.b, wp, dtype, k, vc, ld_w, 64, BK, "w", what))) return rc;
     if ((rc = make_map(&pg.a2, p.d, dtype, vc, m, p.ld_d, 64, BK, "d", what))) return rc;
     if ((rc = make_map(&pg.b2, ra.hc, dtype, k, m, k, 64, BK, "h", what))) return rc;

@@ -286,6 +286,21 @@ def test_pieces_whose_contraction_is_cut(shape, split, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("max_ctas", [1, 2, 3, 7])
+@pytest.mark.parametrize("m", [5, 50, 100])
+def test_few_rows_on_few_ctas(m, max_ctas, cuda_device):
+    """Fewer CTAs than blocks of 256 columns (then the CTA pairs take over), as
+    many, and more; the vocabulary in pieces and in one."""
+    k, v = 600, 3001
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=m, ignored=0.2)
+    dloss = torch.ones(1, device=cuda_device)
+    ref = Ref(h, w, t, _row_g(dloss, t, "sum"))
+    for split in (0, 1024):
+        _, _, dh, dw = _both(h, w, t, dloss, "sum", tune={"max_ctas": max_ctas, "split": split})
+        ref.check_grads(dh, dw)
+
+
+@pytest.mark.gpu
 def test_bands_of_rows(cuda_device):
     """A hidden size whose rows of h fill L2's share in a few row tiles, so the
     logits are walked in several bands."""
