@@ -535,8 +535,8 @@ __device__ __forceinline__ void dh_tile(const CeParams& p, const Tile& t, uint32
 // ---- the CTA-pair kernel ---------------------------------------------------------------
 //
 // Bound by the tensor pipe from some 300 rows up: it is 86-87% active in all three
-// modes at 2048 x 4096 x 65536, where the loss runs 1551 TFLOP/s, d 1516 and the
-// products 1484 in a burst (cuBLAS here: 1583). At hidden sizes of 512 and less the
+// modes at 2048 x 4096 x 65536, where the loss runs 1549 TFLOP/s, d 1521 and the
+// products 1494 in a burst (cuBLAS here: 1583). At hidden sizes of 512 and less the
 // epilogue shows: 3.1 us a tile at k = 64 (reading 128 KB of tensor memory, the
 // exponentials, and the tile's latencies), against 2.2 us of MMA at k = 512.
 
