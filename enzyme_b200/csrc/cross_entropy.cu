@@ -1321,14 +1321,18 @@ __global__ void __launch_bounds__(kStatsThreads) ce_stats(StatsArgs a) {
     }
     sum = warp_sum(sum);
     if (lane == 0) {
-      const float rest = ref + logf(sum);  // the log-sum-exp over the words other than the target
+      const float log_sum = logf(sum);
+      const float rest = ref + log_sum;  // the log-sum-exp over the words other than the target
       float lse = rest, loss = 0.f;
       if (target >= 0) {
         // loss = log(1 + y) with y the other words' odds against the target, so
         // that an almost certain target's loss keeps its digits; past e^80, log y
         const float x = ref - at;
-        if (x > 80.f) {
-          loss = x + logf(sum);
+        if (sum == 0.f) {  // no other word has a probability (v = 1, say)
+          loss = at - at;  // 0, or NaN for an infinite logit
+          lse = at;
+        } else if (x > 80.f) {
+          loss = x + log_sum;
         } else {
           loss = log1pf(sum * expf(x));
           lse = at + loss;

@@ -466,6 +466,33 @@ def test_extreme_logits(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_only_word(dtype, cuda_device):
+    """A vocabulary of one word: its probability is 1 whatever its logit, so the
+    loss and both gradients are 0 and the log-sum-exp is the logit. The same
+    where every other word's logit is -inf."""
+    k = 64
+    at = torch.tensor([-255.0, -100.0, -81.0, -79.0, 0.0, 79.0, 81.0, 100.0, 255.0], device=cuda_device)
+    for m in (len(at), 150):
+        logit = at.repeat(-(-m // len(at)))[:m]
+        h = (logit / 64).to(dtype)[:, None].expand(m, k).contiguous()
+        w = torch.ones(1, k, dtype=dtype, device=cuda_device)
+        t = torch.zeros(m, dtype=torch.int64, device=cuda_device)
+        loss, stats, dh, dw = _both(h, w, t, torch.ones(1, device=cuda_device), "sum")
+        assert float(loss) == 0.0 and not bool(stats[1].any())
+        assert bool(((stats[0] - logit).abs() <= 2 * k * U32 * logit.abs()).all())
+        assert not bool(dh.any()) and not bool(dw.any())
+        # a second word of -inf against rows of positive entries
+        h = h.abs() + 1.0
+        w = torch.full((2, k), -math.inf, dtype=dtype, device=cuda_device)
+        w[0] = -2.0
+        _, stats = ops.linear_cross_entropy(h, w, t)
+        want = -2.0 * h.double().sum(dim=1)
+        assert not bool(stats[1].any())
+        assert bool(((stats[0].double() - want).abs() <= 2 * k * U32 * want.abs()).all())
+
+
+@pytest.mark.gpu
 def test_fp16_scales(cuda_device):
     """fp16 gradients hold at loss scales far from one, and rows of very
     different weight in one call."""
