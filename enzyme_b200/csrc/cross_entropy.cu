@@ -1326,13 +1326,14 @@ __global__ void __launch_bounds__(kStatsThreads) ce_stats(StatsArgs a) {
       float lse = rest, loss = 0.f;
       if (target >= 0) {
         // loss = log(1 + y) with y the other words' odds against the target, so
-        // that an almost certain target's loss keeps its digits; past e^80, log y
-        const float x = ref - at;
+        // that an almost certain target's loss keeps its digits. Past e^80 it is
+        // log y: sum goes up to v, so y leaves fp32's range before exp(x) does.
+        const float x = ref - at, log_y = x + log_sum;
         if (sum == 0.f) {  // no other word has a probability (v = 1, say)
           loss = at - at;  // 0, or NaN for an infinite logit
           lse = at;
-        } else if (x > 80.f) {
-          loss = x + log_sum;
+        } else if (log_y > 80.f) {
+          loss = log_y;
         } else {
           loss = log1pf(sum * expf(x));
           lse = at + loss;

@@ -466,6 +466,31 @@ def test_extreme_logits(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("v", [6000, 32000, 128256])
+@pytest.mark.parametrize("m", [24, 200])  # the narrow and the wide kernels
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_targets_far_below_a_flat_row(dtype, m, v, cuda_device):
+    """Every other word's logit is 0 and the target's is an integer from -66
+    down to -255 (exact in either type): the other words' odds, (v - 1) e^x,
+    pass fp32's range from x = 77 on, the loss does not."""
+    k = 64
+    x = torch.cat([torch.arange(66, 88), torch.tensor([127, 255])]).to(cuda_device)
+    x = x.repeat(-(-m // len(x)))[:m]
+    h = (x / 64).to(dtype)[:, None].expand(m, k).contiguous()
+    assert torch.equal(h.double() * 64, x.double()[:, None].expand(m, k))
+    w = torch.zeros(v, k, dtype=dtype, device=cuda_device)
+    w[v // 2] = -1.0
+    t = torch.full((m,), v // 2, device=cuda_device)
+    dloss = torch.ones(1, device=cuda_device)
+    loss, stats, dh, dw = _both(h, w, t, dloss, "mean")
+    ref = Ref(h, w, t, _row_g(dloss, t, "mean"))
+    assert bool(torch.isfinite(stats).all()) and bool(loss.isfinite())
+    assert abs(float(ref.loss[0]) - 66 - math.log(v - 1)) < 1e-9
+    ref.check_loss(stats)
+    ref.check_grads(dh, dw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_the_only_word(dtype, cuda_device):
     """A vocabulary of one word: its probability is 1 whatever its logit, so the
