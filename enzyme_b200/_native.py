@@ -144,6 +144,10 @@ SIGNATURES: dict[str, tuple] = {
         _I32,
         [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I64, _I32, _P, _I64, _TUNE, _P],
     ),
+    "axon_linear_ce_kept": (
+        _I32,
+        [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I64, _I32, _P, _I64, _TUNE, _P],
+    ),
     "axon_linear_ce_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _TUNE]),
     "axon_linear_ce_grad": (
         _I32,

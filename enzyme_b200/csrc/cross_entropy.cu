@@ -1286,6 +1286,7 @@ struct StatsArgs {
   int m, k, v, parts;
   float* lse;
   float* loss_rows;
+  float* loss_copy;   // the rows' losses a second time, or NULL
   float* loss;        // NULL: no sum or mean asked
   int mean;
   unsigned* done;
@@ -1344,6 +1345,7 @@ __global__ void __launch_bounds__(kStatsThreads) ce_stats(StatsArgs a) {
       }
       a.lse[row] = lse;
       a.loss_rows[row] = loss;
+      if (a.loss_copy) a.loss_copy[row] = loss;
     }
   }
   if (!a.loss) return;
@@ -1866,6 +1868,14 @@ int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse
                    int64_t m, int64_t k, int64_t v, int64_t ld_h, int64_t ld_w, int32_t dtype, int32_t target_bits,
                    int64_t ignore_index, int32_t reduction, void* workspace, int64_t workspace_bytes,
                    const axon_tune_t* tune, void* stream) {
+  return axon_linear_ce_kept(h, w, targets, lse, loss_rows, nullptr, loss, m, k, v, ld_h, ld_w, dtype, target_bits,
+                             ignore_index, reduction, workspace, workspace_bytes, tune, stream);
+}
+
+int axon_linear_ce_kept(const void* h, const void* w, const void* targets, float* lse, float* loss_rows,
+                        float* loss_copy, float* loss, int64_t m, int64_t k, int64_t v, int64_t ld_h, int64_t ld_w,
+                        int32_t dtype, int32_t target_bits, int64_t ignore_index, int32_t reduction, void* workspace,
+                        int64_t workspace_bytes, const axon_tune_t* tune, void* stream) {
   const char* what = "axon_linear_ce";
   axon_tune_t t = tune_or_default(tune);
   int rc = check_head(what, h, w, targets, m, k, v, ld_h, ld_w, dtype, target_bits, reduction, t);
@@ -1896,7 +1906,7 @@ int axon_linear_ce(const void* h, const void* w, const void* targets, float* lse
   p.band = band_of(k);
   if ((rc = logits_maps(what, p, h, ld_h, w, ld_w, dtype))) return rc;
   const StatsArgs a{h, w, ld_h, ld_w, p.part, targets, p.target64, ignore_index, p.m, p.k, p.v, p.parts, lse, loss_rows,
-                    reduction == AXON_REDUCE_NONE ? nullptr : loss, reduction == AXON_REDUCE_MEAN, p.done};
+                    loss_copy, reduction == AXON_REDUCE_NONE ? nullptr : loss, reduction == AXON_REDUCE_MEAN, p.done};
   return dtype == AXON_BF16 ? run_loss<__nv_bfloat16>(p, a, t.max_ctas, s) : run_loss<__half>(p, a, t.max_ctas, s);
 }
 

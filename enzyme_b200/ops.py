@@ -561,18 +561,22 @@ def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", 
     Rows whose target is `ignore_index` have loss 0; any other target outside
     [0, v) gives NaN. Returns (loss, stats): loss the per-row losses ("none"),
     their sum, or their mean over the rows not ignored, in fp32; stats [2, m]
-    fp32 holds each row's log-sum-exp and loss, for linear_cross_entropy_grad."""
+    fp32 holds each row's log-sum-exp and loss, for linear_cross_entropy_grad.
+    The two share no memory: the losses may be weighted or masked in place."""
     m, k, v, ldh, ldw, bits, red = _head_args("linear_cross_entropy", h, w, targets, reduction, workspace)
     lib, dev = N.lib(), h.device
     with _on_device(dev):
-        res = torch.empty(2 * m + 1, dtype=torch.float32, device=dev)
+        # log-sum-exps, the rows' losses, and what is returned as the loss
+        each = red == N.AXON_REDUCE_NONE
+        res = torch.empty(2 * m + (m if each else 1), dtype=torch.float32, device=dev)
         at = res.data_ptr()
         ws = _workspace(_check_ws_bytes(lib.axon_linear_ce_workspace_bytes(m, k, v)), dev, workspace)
-        check(lib.axon_linear_ce(h.data_ptr(), w.data_ptr(), targets.data_ptr(), at, at + 4 * m, at + 8 * m, m, k, v,
-                                 ldh, ldw, dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.nbytes,
-                                 _tune(tune), _stream(h)))
+        check(lib.axon_linear_ce_kept(h.data_ptr(), w.data_ptr(), targets.data_ptr(), at, at + 4 * m,
+                                      at + 8 * m if each else None, None if each else at + 8 * m, m, k, v, ldh, ldw,
+                                      dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.nbytes,
+                                      _tune(tune), _stream(h)))
     stats = res.as_strided((2, m), (m, 1))
-    return stats[1] if red == N.AXON_REDUCE_NONE else res[2 * m], stats
+    return res[2 * m:] if each else res[2 * m], stats
 
 
 def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100, reduction="mean", need=(True, True),

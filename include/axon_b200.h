@@ -344,6 +344,16 @@ AXON_API int axon_linear_ce(const void* h, const void* w, const void* targets, f
                             int64_t ignore_index, int32_t reduction, void* workspace,
                             int64_t workspace_bytes, const axon_tune_t* tune, void* stream);
 
+/* axon_linear_ce with the rows' losses written a second time, to loss_copy [m]
+ * (NULL: axon_linear_ce): for a caller that hands the losses on to code that may
+ * change them, while loss_rows is kept as it is for axon_linear_ce_grad. */
+AXON_API int axon_linear_ce_kept(const void* h, const void* w, const void* targets, float* lse,
+                                 float* loss_rows, float* loss_copy, float* loss, int64_t m, int64_t k,
+                                 int64_t v, int64_t ld_h, int64_t ld_w, int32_t dtype,
+                                 int32_t target_bits, int64_t ignore_index, int32_t reduction,
+                                 void* workspace, int64_t workspace_bytes, const axon_tune_t* tune,
+                                 void* stream);
+
 /* Gradients for the same operands: with g_i = dloss[i] (AXON_REDUCE_NONE),
  * dloss[0] (SUM) or dloss[0] / counted rows (MEAN), dloss fp32 on the device,
  *   d_ij = g_i (exp(s_ij - lse_i) - [j = targets[i]]), dh = d w, dw = d^T h.

@@ -95,6 +95,15 @@ def test_more_refusals():
         assert _bwd(**kw) == code, (kw, N.last_error())
 
 
+def test_the_form_with_a_copy_refuses_the_same():
+    for kw in (dict(rows=None), dict(k=60), dict(dt=N.AXON_F32), dict(ws=None)):
+        a = dict(rows=FAKE, k=64, dt=N.AXON_BF16, ws=FAKE)
+        a.update(kw)
+        rc = N.lib().axon_linear_ce_kept(FAKE, FAKE, FAKE, FAKE, a["rows"], FAKE, None, 4, a["k"], 100, 64, 64, a["dt"],
+                                         64, IGNORE, N.AXON_REDUCE_NONE, a["ws"], BIG, None, None)
+        assert rc == _fwd(red=N.AXON_REDUCE_NONE, **kw) != N.AXON_OK
+
+
 def test_outputs_over_operands_are_refused():
     """dh and dw are written while the operands are read. Addresses far apart
     for everything but the pair under test (nothing is dereferenced)."""
@@ -266,6 +275,27 @@ def test_gradients(shape, dtype, reduction, cuda_device):
     ref.check_loss(stats)
     ref.check_grads(dh, dw)
     assert not bool(dh[~ref.keep].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_losses_changed_in_place(m, cuda_device):
+    """The per-row losses are the caller's: what is done to them between the
+    two calls reaches neither stats nor the gradients."""
+    k, v = 64, 700
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=m)
+    dloss = torch.ones(m, device=cuda_device)
+    loss, stats, dh, dw = _both(h, w, t, dloss, "none")
+    kept = stats.clone()
+    assert torch.equal(loss, stats[1])
+    loss *= 0
+    assert torch.equal(stats, kept)
+    dh2, dw2 = ops.linear_cross_entropy_grad(h, w, t, stats, dloss, reduction="none")
+    assert torch.equal(dh, dh2) and torch.equal(dw, dw2)
+    # and the other way round
+    loss, stats = ops.linear_cross_entropy(h, w, t, reduction="none")
+    stats.zero_()
+    assert torch.equal(loss, kept[1])
 
 
 @pytest.mark.gpu
