@@ -553,6 +553,16 @@ def _head_args(name, h, w, targets, reduction, workspace):
     return m, k, v, ldh if m > 1 else k, ldw if v > 1 else k, bits, red
 
 
+def _head_out(name, t, like, types) -> int:
+    """Checks a tensor that takes the gradient of `like`; its leading dimension."""
+    if t is None:
+        return like.shape[1]
+    if t.shape != like.shape or t.dtype not in types or t.device != like.device:
+        raise N.AxonError(N.AXON_E_ARG, f"{name}: out must have the operands' shapes and types")
+    rows, cols, ld = _rows(t)  # a single row's elements lie side by side too
+    return ld if rows > 1 else cols
+
+
 def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", workspace=None, tune=None):
     """Softmax cross entropy of the logits h @ w.T, which are never stored.
 
@@ -601,13 +611,8 @@ def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100,
     lddh = lddw = k
     if out is not None:
         dh, dw = out
-        for t, like, types in ((dh, h, (h.dtype,)), (dw, w, (w.dtype, torch.float32))):
-            if t is not None and (t.shape != like.shape or t.dtype not in types or t.device != dev):
-                raise N.AxonError(N.AXON_E_ARG, f"{name}: out must have the operands' shapes and types")
-        if dh is not None and m > 1:
-            lddh = _rows(dh)[2]
-        if dw is not None and v > 1:
-            lddw = _rows(dw)[2]
+        lddh = _head_out(name, dh, h, (h.dtype,))
+        lddw = _head_out(name, dw, w, (w.dtype, torch.float32))
     elif dw_dtype not in (None, w.dtype, torch.float32):
         raise N.AxonError(N.AXON_E_ARG, f"{name}: dw has w's type or fp32")
     with _on_device(dev):

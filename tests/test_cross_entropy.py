@@ -146,6 +146,26 @@ def test_host_tensors_are_refused():
     assert e.value.code == N.AXON_E_ARG and "CUDA" in e.value.message
 
 
+@pytest.mark.parametrize("rows", [1, 2, 7])
+def test_outputs_whose_rows_are_not_contiguous_are_refused(rows):
+    """k elements are written from a row's start, in a single row as in many:
+    every second element, a column and an expanded row are no such memory."""
+    like = torch.zeros(rows, 16).bfloat16()
+    room = torch.zeros(64, 64).bfloat16()
+    for t in (room[:rows, :32:2], room[:16, :rows].T, room[:rows, :1].expand(rows, 16)):
+        assert t.shape == like.shape
+        with pytest.raises(N.AxonError) as e:
+            ops._head_out("f", t, like, (torch.bfloat16,))
+        assert e.value.code == N.AXON_E_SHAPE
+    for t in (room[:rows].float()[:, :16], room[:rows, :8]):
+        with pytest.raises(N.AxonError) as e:
+            ops._head_out("f", t, like, (torch.bfloat16,))
+        assert e.value.code == N.AXON_E_ARG
+    ld = 64 if rows > 1 else 16
+    assert ops._head_out("f", room[:rows, 16:32], like, (torch.bfloat16,)) == ld
+    assert ops._head_out("f", None, like, (torch.bfloat16,)) == 16
+
+
 # ---- GPU ----------------------------------------------------------------------------
 
 
@@ -373,6 +393,30 @@ def test_strides_types_and_parts(cuda_device):
     assert none is None and torch.equal(dh2, dh)
     _, _, none, dw2 = _both(h, w, t, dloss, "mean", need=(False, True), dw_dtype=torch.float32)
     assert none is None and torch.equal(dw2, dw)
+
+
+@pytest.mark.gpu
+def test_outputs_of_a_single_row(cuda_device):
+    """m = 1 and v = 1: outputs inside a larger buffer are written and nothing
+    beside them; ones whose elements do not lie side by side are refused."""
+    k = 64
+    one = torch.ones(1, device=cuda_device)
+    for m, v in ((1, 9), (9, 1)):
+        h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=m)
+        _, stats, dh, dw = _both(h, w, t, one, "sum")
+        room = torch.full((40, 2 * k + 8), 7.0, dtype=torch.bfloat16, device=cuda_device)
+        _both(h, w, t, one, "sum", out=(room[:m, 8:8 + k], room[20:20 + v, 8:8 + k]))
+        assert torch.equal(room[:m, 8:8 + k], dh) and torch.equal(room[20:20 + v, 8:8 + k], dw)
+        rest = room.clone()
+        rest[:m, 8:8 + k] = rest[20:20 + v, 8:8 + k] = 7.0
+        assert bool((rest == 7).all())
+        before = room.clone()
+        for bad_h, bad_w in ((room[:m, :2 * k:2], torch.empty_like(w)), (torch.empty_like(h), room[:v, :2 * k:2]),
+                             (room[:m, :1].expand(m, k), None), (None, room[:v, :1].expand(v, k))):
+            with pytest.raises(N.AxonError) as e:
+                ops.linear_cross_entropy_grad(h, w, t, stats, one, reduction="sum", out=(bad_h, bad_w))
+            assert e.value.code == N.AXON_E_SHAPE
+        assert torch.equal(room, before)
 
 
 @pytest.mark.gpu
