@@ -553,6 +553,17 @@ def _head_args(name, h, w, targets, reduction, workspace):
     return m, k, v, ldh if m > 1 else k, ldw if v > 1 else k, bits, red
 
 
+def _head_workspace(nbytes: int, device, workspace=None) -> torch.Tensor:
+    """A workspace of one block of memory: the given one, of any type, or a new one."""
+    if workspace is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if not workspace.is_contiguous():
+        raise N.AxonError(N.AXON_E_SHAPE, "workspace must be contiguous")
+    if workspace.nbytes < nbytes:
+        raise N.AxonError(N.AXON_E_ARG, f"workspace of {nbytes} bytes needed")
+    return workspace
+
+
 def _head_out(name, t, like, types) -> int:
     """Checks a tensor that takes the gradient of `like`; its leading dimension."""
     if t is None:
@@ -580,7 +591,7 @@ def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", 
         each = red == N.AXON_REDUCE_NONE
         res = torch.empty(2 * m + (m if each else 1), dtype=torch.float32, device=dev)
         at = res.data_ptr()
-        ws = _workspace(_check_ws_bytes(lib.axon_linear_ce_workspace_bytes(m, k, v)), dev, workspace)
+        ws = _head_workspace(_check_ws_bytes(lib.axon_linear_ce_workspace_bytes(m, k, v)), dev, workspace)
         check(lib.axon_linear_ce_kept(h.data_ptr(), w.data_ptr(), targets.data_ptr(), at, at + 4 * m,
                                       at + 8 * m if each else None, None if each else at + 8 * m, m, k, v, ldh, ldw,
                                       dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.nbytes,
@@ -620,7 +631,7 @@ def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100,
             dh = torch.empty((m, k), dtype=h.dtype, device=dev) if need[0] else None
             dw = torch.empty((v, k), dtype=dw_dtype or w.dtype, device=dev) if need[1] else None
         tune_ref = _tune(tune)
-        ws = _workspace(_check_ws_bytes(lib.axon_linear_ce_grad_workspace_bytes(m, k, v, tune_ref)), dev, workspace)
+        ws = _head_workspace(_check_ws_bytes(lib.axon_linear_ce_grad_workspace_bytes(m, k, v, tune_ref)), dev, workspace)
         at = stats.data_ptr()
         check(lib.axon_linear_ce_grad(h.data_ptr(), w.data_ptr(), targets.data_ptr(), at, at + 4 * m, dloss.data_ptr(),
                                       _ptr(dh), _ptr(dw), m, k, v, ldh, ldw, lddh, lddw, dtype_code(h),

@@ -146,6 +146,23 @@ def test_host_tensors_are_refused():
     assert e.value.code == N.AXON_E_ARG and "CUDA" in e.value.message
 
 
+def test_workspaces_that_are_no_block_of_memory_are_refused():
+    """An expanded tensor has its bytes in its shape only, a strided one in
+    between others' elements; what counts is bytes, not elements."""
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(4096), torch.zeros(8192, dtype=torch.uint8)[::2],
+               torch.zeros(64, 64, dtype=torch.uint8).T):
+        with pytest.raises(N.AxonError) as e:
+            ops._head_workspace(4096, ws.device, ws)
+        assert e.value.code == N.AXON_E_SHAPE
+    with pytest.raises(N.AxonError) as e:
+        ops._head_workspace(4096, "cpu", torch.zeros(4095, dtype=torch.uint8))
+    assert e.value.code == N.AXON_E_ARG and "4096 bytes" in e.value.message
+    for dtype in (torch.uint8, torch.float32):
+        ws = torch.zeros(4096, dtype=torch.uint8).view(dtype)
+        assert ops._head_workspace(4096, "cpu", ws) is ws
+    assert ops._head_workspace(4096, "cpu").nbytes == 4096
+
+
 @pytest.mark.parametrize("rows", [1, 2, 7])
 def test_outputs_whose_rows_are_not_contiguous_are_refused(rows):
     """k elements are written from a row's start, in a single row as in many:
@@ -760,3 +777,26 @@ def test_wrapper_refusals(cuda_device):
     assert code(lambda: grad(h, w, t, stats, one, out=(h[:2], w))) == N.AXON_E_ARG
     assert code(lambda: grad(h, w, t, stats, one, out=(h, torch.empty_like(w)))) == N.AXON_E_ARG
     assert code(lambda: grad(h, w, t, stats, one, out=(torch.empty_like(h), w))) == N.AXON_E_ARG
+
+
+@pytest.mark.gpu
+def test_given_workspaces(cuda_device):
+    """A caller's workspace, of bytes or of another type, gives the same bits;
+    one that is no block of memory is refused before anything is launched."""
+    h, w, t = _inputs(cuda_device, 40, 64, 500, torch.bfloat16, seed=3, ignored=0.1)
+    one = torch.ones(1, device=cuda_device)
+    want = _both(h, w, t, one, "mean")
+    need = max(N.lib().axon_linear_ce_workspace_bytes(40, 64, 500),
+               N.lib().axon_linear_ce_grad_workspace_bytes(40, 64, 500, None))
+    for ws in (torch.empty(need, dtype=torch.uint8, device=cuda_device),
+               torch.full((need // 4,), float("nan"), device=cuda_device)):
+        loss, stats = ops.linear_cross_entropy(h, w, t, workspace=ws)
+        dh, dw = ops.linear_cross_entropy_grad(h, w, t, stats, one, workspace=ws)
+        for a, b in zip((loss, stats, dh, dw), want):
+            assert torch.equal(a, b)
+    flat = torch.zeros(1, dtype=torch.uint8, device=cuda_device).expand(need)
+    for call in (lambda: ops.linear_cross_entropy(h, w, t, workspace=flat),
+                 lambda: ops.linear_cross_entropy_grad(h, w, t, want[1], one, workspace=flat)):
+        with pytest.raises(N.AxonError) as e:
+            call()
+        assert e.value.code == N.AXON_E_SHAPE
