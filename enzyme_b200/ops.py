@@ -641,4 +641,6 @@ def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100,
 
 
 def linear_cross_entropy_status(device=None) -> None:
-    check(N.lib().axon_linear_ce_status(torch.cuda.current_stream(device).cuda_stream))
+    # the word that is read is the current device's
+    with torch.cuda.device(device):
+        check(N.lib().axon_linear_ce_status(torch.cuda.current_stream().cuda_stream))

@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import types
 
 import pytest
 import torch
@@ -161,6 +162,33 @@ def test_workspaces_that_are_no_block_of_memory_are_refused():
         ws = torch.zeros(4096, dtype=torch.uint8).view(dtype)
         assert ops._head_workspace(4096, "cpu", ws) is ws
     assert ops._head_workspace(4096, "cpu").nbytes == 4096
+
+
+def test_status_of_another_device_is_asked_there(monkeypatch):
+    """The status word belongs to the current device: it has to be the one whose
+    stream is waited for."""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, device):
+            self.to = current[0] if device is None else device
+
+        def __enter__(self):
+            self.back, current[0] = current[0], self.to
+
+        def __exit__(self, *exc):
+            current[0] = self.back
+
+    def stream(device=None):
+        return types.SimpleNamespace(cuda_stream=100 + (current[0] if device is None else device))
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", stream)
+    monkeypatch.setattr(N, "lib", lambda: types.SimpleNamespace(
+        axon_linear_ce_status=lambda s: seen.append((current[0], s)) or 0))
+    for device in (None, 1):
+        ops.linear_cross_entropy_status(device)
+    assert seen == [(0, 100), (1, 101)] and current == [0]
 
 
 @pytest.mark.parametrize("rows", [1, 2, 7])
