@@ -230,10 +230,11 @@ class GradList:
     they come, empty ones allowed, each dense in memory (any order of its
     dimensions). `out`, where clip_grads writes, is None (in place) or a list of
     tensors that match them in shape, type and strides and overlap nothing else
-    in the two lists. The tensors are held; one whose memory has moved
-    since (`set_`, `.data =`, a storage resize) makes the next call raise."""
+    in the two lists. The tensors and the memory they have now are held, with
+    their sizes and types of now; one whose memory has moved since (`set_`,
+    `.data =`, a storage resize) makes the next call raise."""
 
-    def __init__(self, grads, out=None):
+    def __init__(self, grads, out=None, *, _keep=True):
         self.grads = list(grads)
         self.out = self.grads if out is None else list(out)
         if not self.grads:
@@ -253,6 +254,10 @@ class GradList:
         n = len(self.grads)
         self._where = [t.data_ptr() for t in self.grads]
         self._where_out = [t.data_ptr() for t in self.out]
+        if _keep:
+            # while it is held, the old memory of a tensor that moves is not given
+            # to another: an address that is still the same is still this memory
+            self._memory = [t.untyped_storage() for ts in (self.grads, self.out) for t in ts]
         self._in_ptrs = (ctypes.c_void_p * n)(*self._where)
         self._out_ptrs = (ctypes.c_void_p * n)(*self._where_out)
         self._sizes = (ctypes.c_int64 * n)(*(t.numel() for t in self.grads))
@@ -305,7 +310,7 @@ def _grad_list(grads, out=None) -> GradList:
         if out is not None:
             raise N.AxonError(N.AXON_E_ARG, "gradient list: a GradList has its own out")
         return grads
-    return GradList(grads, out=out)
+    return GradList(grads, out=out, _keep=False)  # for one call
 
 
 def _on_device(device):

@@ -284,6 +284,28 @@ def test_list_refusals(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("which", ["grads", "out"])
+def test_memory_that_is_freed_is_not_taken_for_the_list(which, cuda_device):
+    """A listed tensor gives its memory up and gets a smaller one of the same
+    kind, which an allocator would serve from the block just freed: the list
+    holds that block, so the address differs and the call raises."""
+    n = 1 << 20
+    x, o = torch.ones(n, device=cuda_device), torch.zeros(n, device=cuda_device)
+    lst = ops.GradList([x], out=[o])
+    ops.clip_grads(lst, 1.0)
+    t = x if which == "grads" else o
+    was = t.data_ptr()
+    torch.cuda.synchronize()
+    for size in (n, n // 2, 100):
+        t.data = torch.empty(0, device=cuda_device)
+        t.data = torch.ones(size, device=cuda_device)
+        assert t.data_ptr() != was
+        with pytest.raises(N.AxonError) as e:
+            ops.clip_grads(lst, 1.0)
+        assert e.value.code == N.AXON_E_ARG and "moved" in e.value.message
+
+
+@pytest.mark.gpu
 def test_other_stream_and_graph(cuda_device):
     """On a side stream, and captured: two graphs of one list replayed with
     other values each time."""
