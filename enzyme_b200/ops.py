@@ -241,7 +241,10 @@ class GradList:
             raise N.AxonError(N.AXON_E_SHAPE, "gradient list: empty (no device to work on)")
         if len(self.out) != len(self.grads):
             raise N.AxonError(N.AXON_E_SHAPE, "gradient list: out must have a tensor for each gradient")
-        _require_cuda(*self.grads, *self.out)
+        for t in self.grads if self.out is self.grads else (*self.grads, *self.out):
+            if t is None:
+                raise N.AxonError(N.AXON_E_ARG, "gradient list: None (leave parameters without a gradient out)")
+            _require_cuda(t)
         self.device = self.grads[0].device
         for t, o in zip(self.grads, self.out):
             if t.device != self.device or o.device != self.device:

@@ -87,6 +87,15 @@ def test_grad_lists_on_the_host_are_refused():
     assert e.value.code == N.AXON_E_ARG and "CUDA" in e.value.message
 
 
+def test_parameters_without_a_gradient_are_refused():
+    x = torch.zeros(4)
+    for call in (lambda: ops.grad_norm([None]), lambda: ops.grad_norm_scale([None, x], 1.0),
+                 lambda: ops.clip_grads([None, x], 1.0), lambda: ops.GradList([None], out=[x])):
+        with pytest.raises(N.AxonError) as e:
+            call()
+        assert e.value.code == N.AXON_E_ARG and "None" in e.value.message
+
+
 def test_dense_memory_in_any_order():
     t = torch.zeros(4, 6, 5)
     assert ops._is_dense(t) and ops._is_dense(t.permute(2, 0, 1)) and ops._is_dense(torch.zeros(()))
