@@ -244,7 +244,8 @@ class GradList:
         for t in self.grads if self.out is self.grads else (*self.grads, *self.out):
             if t is None:
                 raise N.AxonError(N.AXON_E_ARG, "gradient list: None (leave parameters without a gradient out)")
-            _require_cuda(t)
+            if not t.is_cuda:
+                _require_cuda(t)
         self.device = self.grads[0].device
         for t, o in zip(self.grads, self.out):
             if t.device != self.device or o.device != self.device:
