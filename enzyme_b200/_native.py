@@ -156,6 +156,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "axon_linear_ce_status": (_I32, [_P]),
     "axon_cast": (_I32, [_P, _P, _I64, _I32, _I32, _P]),
+    "axon_selftest_linear_ce_gave_up": (_I32, [_P]),
     "axon_selftest_bounded_wait": (_I32, [_I64, _P, _P, _P]),
     "axon_row_rsqrt": (_I32, [_P, _P, _I64, _I64, _I64, _I32, _F, _F, _P]),
     "axon_row_status": (_I32, [_P]),

@@ -76,7 +76,7 @@ constexpr int smem_of(int mode) { return stages_of(mode) * STAGE + staging_of(mo
 // What ce_grad_rows hands to the kernels after it.
 struct RowHeader {
   int rows;         // rows that count
-  float unscale;    // what d must be multiplied by
+  float unscale;    // what d must be multiplied by (see products_scale)
 };
 
 struct CeParams {
@@ -134,6 +134,11 @@ __device__ __forceinline__ float exp_from(float x, float ref) { return ex2((x - 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_ce_error));
 }
+
+// Whether a wait gave up before this kernel (and nobody has asked for the status
+// since): what the workspace holds is then not to be trusted, and the kernels
+// that form the results write NaN. Asked once a thread, after pdl_wait.
+__device__ __forceinline__ bool gave_up() { return *static_cast<volatile int*>(&g_ce_error) != 0; }
 
 // ---- tiles -----------------------------------------------------------------------------
 
@@ -279,6 +284,11 @@ __device__ __forceinline__ uint32_t idesc(int n, bool a_mn, bool b_mn, int m = 2
 }
 
 // ---- epilogues -----------------------------------------------------------------------
+
+// What the products of d are multiplied by.
+__device__ __forceinline__ float products_scale(const RowHeader* header) {
+  return gave_up() ? __int_as_float(0x7fc00000) : header->unscale;
+}
 
 // COLS accumulator columns from tensor memory.
 template <int COLS>
@@ -657,7 +667,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant
   } else if (warp >= 2) {
     // ---------------- epilogue (both CTAs, their own 128 rows) ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    const float unscale = MODE == kGrads ? p.header->unscale : 1.f;
+    const float unscale = MODE == kGrads ? products_scale(p.header) : 1.f;
     uint32_t turn = 0;
     for (int i = 0; w.at(p, i, t); ++i) {
       const int buf = i & 1;
@@ -955,7 +965,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few(const __grid_constant__
   } else if (warp >= 12) {
     // ---------------- dh: epilogue ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    const float unscale = p.header->unscale;
+    const float unscale = products_scale(p.header);
     int i = 0;
     for (int t = blockIdx.x; t < n_dh; t += gridDim.x, ++i) {
       const int buf = i & 1;
@@ -969,7 +979,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few(const __grid_constant__
   } else if (warp >= 4) {
     // ---------------- dw: epilogue ----------------
     const int q = warp & 3, c0 = warp < 8 ? 0 : BN / 2;
-    const float unscale = p.header->unscale;
+    const float unscale = products_scale(p.header);
     uint8_t* stg = staging + (warp - 4) * BUFS * kStaging;
     uint32_t use = 0, turn = 0;
     for (int tm = tm0; tm < word_tiles; tm += step, use ^= 1u) {
@@ -1343,6 +1353,7 @@ __global__ void __launch_bounds__(kStatsThreads) ce_stats(StatsArgs a) {
       } else if (target == -2) {
         loss = __int_as_float(0x7fc00000);
       }
+      if (gave_up()) lse = loss = __int_as_float(0x7fc00000);
       a.lse[row] = lse;
       a.loss_rows[row] = loss;
       if (a.loss_copy) a.loss_copy[row] = loss;
@@ -1487,7 +1498,7 @@ __global__ void __launch_bounds__(256) ce_dh_finish(const float* __restrict__ ac
   pdl_wait();
   pdl_trigger();
   const int64_t groups = static_cast<int64_t>(header->rows) * (k / 8);
-  const float unscale = header->unscale;
+  const float unscale = products_scale(header);
   const int part = threadIdx.x & 3;
   // all lanes of a warp take the same number of rounds: they exchange sums
   for (int64_t i0 = blockIdx.x * 64ll; i0 < groups; i0 += gridDim.x * 64ll) {
@@ -2029,6 +2040,14 @@ int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const
       return rc;
   }
   return AXON_OK;
+}
+
+int axon_selftest_linear_ce_gave_up(void* stream) {
+  const int code = AXON_E_TIMEOUT;
+  cudaStream_t s = as_stream(stream);
+  cudaError_t e = cudaMemcpyToSymbolAsync(g_ce_error, &code, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  return e == cudaSuccess ? AXON_OK : fail(AXON_E_CUDA, "axon_selftest_linear_ce_gave_up: %s", cudaGetErrorString(e));
 }
 
 int axon_linear_ce_status(void* stream) {

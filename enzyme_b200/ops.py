@@ -650,6 +650,8 @@ def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100,
 
 
 def linear_cross_entropy_status(device=None) -> None:
+    """Raise AxonError(AXON_E_TIMEOUT) if a bounded wait of linear_cross_entropy or
+    its gradient gave up since the last query; until then results are NaN."""
     # the word that is read is the current device's
     with torch.cuda.device(device):
         check(N.lib().axon_linear_ce_status(torch.cuda.current_stream().cuda_stream))

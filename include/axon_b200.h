@@ -377,7 +377,10 @@ AXON_API int axon_linear_ce_grad(const void* h, const void* w, const void* targe
                                  void* stream);
 
 /* Synchronise `stream` and report whether one of the two calls since the last
- * query gave up on a bounded pipeline wait (AXON_E_TIMEOUT; then cleared). */
+ * query gave up on a bounded pipeline wait (AXON_E_TIMEOUT; then cleared).
+ * From the wait that gave up until this query, losses, log-sum-exps and
+ * gradients come out as NaN; of the gradients that were being formed when it
+ * gave up, some may be what their memory held before. */
 AXON_API int axon_linear_ce_status(void* stream);
 
 /* ---- tensor-parallel SwiGLU over NVLink peer memory ----------------------- */
@@ -540,6 +543,11 @@ AXON_API int axon_cast(const void* src, void* dst, int64_t n, int32_t src_dtype,
  * receives AXON_E_TIMEOUT for each wait that gave up (AXON_OK if the flag was
  * set). Lets tests check the timeout path on a GPU without a fault or hang. */
 AXON_API int axon_selftest_bounded_wait(int64_t limit_ns, void* status2, const void* flag, void* stream);
+
+/* Diagnostic: leaves the current device as a wait of axon_linear_ce that gave up
+ * leaves it, without one (synchronises `stream`). Lets tests check what the
+ * calls after it return and that axon_linear_ce_status reports and clears it. */
+AXON_API int axon_selftest_linear_ce_gave_up(void* stream);
 
 /* Per-row scale r[i] = rsqrt(scale * sum_j x[i,j]^2 + eps) in fp32: the norm
  * prologue of rmsnorm_matmul (Axon kernels/rmsnorm_matmul/refs.py:16-22) and

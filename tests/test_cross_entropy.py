@@ -808,6 +808,28 @@ def test_wrapper_refusals(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [5, 100, 300])
+def test_after_a_wait_gave_up(m, cuda_device):
+    """Results are NaN, not whatever the workspace held, until the status has
+    been asked for; then they are the same bits as before."""
+    h, w, t = _inputs(cuda_device, m, 64, 1500, torch.bfloat16, seed=m)
+    one = torch.ones(1, device=cuda_device)
+    want = _both(h, w, t, one, "mean")
+    stream = torch.cuda.current_stream().cuda_stream
+    for tune in (None, {"split": 512}):
+        assert N.lib().axon_selftest_linear_ce_gave_up(stream) == N.AXON_OK, N.last_error()
+        loss, stats = ops.linear_cross_entropy(h, w, t)
+        dh, dw = ops.linear_cross_entropy_grad(h, w, t, want[1], one, tune=tune)
+        for x in (loss, stats, dh, dw):
+            assert bool(x.isnan().all())
+        with pytest.raises(N.AxonError) as e:
+            ops.linear_cross_entropy_status(cuda_device)
+        assert e.value.code == N.AXON_E_TIMEOUT
+        for a, b in zip(_both(h, w, t, one, "mean"), want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_given_workspaces(cuda_device):
     """A caller's workspace, of bytes or of another type, gives the same bits;
     one that is no block of memory is refused before anything is launched."""
