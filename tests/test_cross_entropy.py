@@ -610,6 +610,33 @@ def test_targets_far_below_a_flat_row(dtype, m, v, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [5, 200])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_an_almost_certain_target_keeps_its_digits(dtype, m, cuda_device):
+    """The target's logit is a sum in fp32 lanes, not the tensor core's. Every
+    other word's logit is 0 exactly, so the loss log(1 + (v - 1) e^-s) is off by
+    the error of s and, relative to itself, by that of expf, a product and
+    log1pf (4 ulp in all, 8 half steps). s: products exact in fp32; a lane adds
+    k / 256 = 16 of them one after the other, on average onto half of its sum at
+    most where no term is negative, and 8 more additions join lanes: 16 / 2 +
+    1 + 8 = 17 half steps of the sum. With s of 7 to 13 that is 1.3e-5 at
+    most; the tensor core's sum of these (256 steps, each cut off and not
+    rounded) is 1.0e-4 off in bf16 and 2.5e-4 in fp16."""
+    k, v = 4096, 1000
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    h = (0.5 + torch.rand(m, k, device=cuda_device, generator=g)).to(dtype)
+    w = torch.zeros(v, k, dtype=dtype, device=cuda_device)
+    w[7] = ((0.5 + torch.rand(k, device=cuda_device, generator=g)) * (10.0 / k)).to(dtype)
+    t = torch.full((m,), 7, device=cuda_device)
+    s = h.double() @ w[7].double()
+    assert bool((s > 7).all()) and bool((s < 13).all())
+    want = torch.log1p((v - 1) * torch.exp(-s))
+    loss, stats = ops.linear_cross_entropy(h, w, t, reduction="none")
+    assert bool(((loss.double() - want).abs() <= (17 * s + 8) * U32 * want).all())
+    assert bool(((stats[0].double() - s - want).abs() <= (17 * s + 8 * want + s + want) * U32).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_the_only_word(dtype, cuda_device):
     """A vocabulary of one word: its probability is 1 whatever its logit, so the
