@@ -104,7 +104,7 @@ struct CeParams {
   const int* row_index; // counted row -> row of dh
   void* dh;
   void* dw;
-  int64_t ld_dh, ld_dw;
+  int64_t ld_dh;
   float* acc;           // fp32 [splits][m][k]: dh between pieces, and its splits
   int first, last;      // this piece is the vocabulary's first / last
   int splits;           // parts that dh's contraction over the piece is cut into
@@ -1308,7 +1308,8 @@ constexpr int kStatsRows = kStatsThreads / 32;
 // Joins a row's (max, sum) parts with the target's logit, a warp per row (27 us
 // for 4096 rows of k = 4096, most of it the targets' rows of w); the
 // CTA that comes last adds the rows' losses up, in row order whichever CTA it
-// is.
+// is, with its 128 threads: that sum grows with m alone (230 us for 131072 rows of
+// k = 64, most of it this sum; a head of 4096 x 128256 takes some 90 ms for them).
 template <typename T>
 __global__ void __launch_bounds__(kStatsThreads) ce_stats(StatsArgs a) {
   const float ninf = __int_as_float(0xff800000);
@@ -1408,9 +1409,10 @@ constexpr int kRowThreads = 256;
 
 // Moves the rows that count to the front. Every CTA owns a range of rows; it
 // finds the number of counted rows before its own, and the largest |g|, by
-// reading all targets itself: m is at most some ten thousands, and a second
-// launch would cost more. Bound by the copy of h: 18 us at 4096 x 4096, 6 at 64
-// rows.
+// reading all targets itself, where a second launch would cost more. Bound by the
+// copy of h: 18 us at 4096 x 4096, 6 at 64 rows. The reads of the targets (and of
+// dloss, one a row) grow with m times the CTAs, four an SM at most, from L2:
+// 117 us in all for 131072 rows of k = 64, where d and its products take 845.
 __global__ void __launch_bounds__(kRowThreads) ce_grad_rows(RowsArgs a) {
   __shared__ int slot[kRowThreads];
   __shared__ int warp_count[kRowThreads / 32];
@@ -2012,7 +2014,6 @@ int axon_linear_ce_grad(const void* h, const void* w, const void* targets, const
     p.dh = dh;
     p.dw = dw;
     p.ld_dh = ld_dh;
-    p.ld_dw = ld_dw;
     p.acc = reinterpret_cast<float*>(ws + g.off_acc);
     p.first = i == 0;
     p.last = i + 1 == g.pieces;

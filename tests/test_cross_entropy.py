@@ -716,6 +716,26 @@ def test_wider_head(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,split", [(4097, 0), (70001, 0), (70001, 256)])
+def test_many_rows(m, split, cuda_device):
+    """Rows past a padded batch's: more row tiles than pairs, many rows a CTA in
+    the kernels that join and move rows, the vocabulary in one piece and three."""
+    k, v = 64, 700
+    h, w, t = _inputs(cuda_device, m, k, v, torch.bfloat16, seed=m, ignored=0.3)
+    t[:300] = IGNORE
+    t[-1] = v - 1
+    dloss = torch.randn(m, device=cuda_device, generator=torch.Generator(device=cuda_device).manual_seed(1))
+    loss, stats, dh, dw = _both(h, w, t, dloss, "none", tune={"split": split})
+    ref = Ref(h, w, t, dloss)
+    ref.check_loss(stats)
+    ref.check_grads(dh, dw)
+    assert torch.equal(loss, stats[1]) and not bool(dh[~ref.keep].any())
+    mean, _ = ops.linear_cross_entropy(h, w, t)
+    want = float(stats[1].double().sum() / ref.keep.sum())
+    assert abs(float(mean) - want) <= 2 * U32 * want
+
+
+@pytest.mark.gpu
 def test_other_stream_and_graph(cuda_device):
     """On a side stream, and captured twice with replays on new values."""
     m, k, v = 200, 128, 1500
