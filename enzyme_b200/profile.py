@@ -214,6 +214,17 @@ def case_linear_ce_grad(gen):
     return lambda: ops.linear_cross_entropy_grad(h, w, t, stats, one)
 
 
+def case_linear_ce_grad_few(gen):
+    """ce_few: both products of 64 rows, k 4096, v 65536 (0.5 GB of w read, of dw
+    written)."""
+    from . import ops
+
+    h, w, t = _head(gen, 64, 65536)
+    _, stats = ops.linear_cross_entropy(h, w, t)
+    one = torch.ones(1, device="cuda")
+    return lambda: ops.linear_cross_entropy_grad(h, w, t, stats, one)
+
+
 def case_linear_ce_token(gen):
     """ce_narrow: one row against 128256 words of 4096 (1.05 GB streamed)."""
     from . import ops
@@ -246,6 +257,7 @@ CASES = {
     "softmax_cta": (case_softmax_cta, "row_cta_bulk_kernel"),
     "linear_ce": (case_linear_ce, "ce_pair"),
     "linear_ce_grad": (case_linear_ce_grad, "ce_pair"),
+    "linear_ce_grad_few": (case_linear_ce_grad_few, "ce_few"),
     "linear_ce_token": (case_linear_ce_token, "ce_narrow"),
     "grad_clip": (case_grad_clip, "grad_scale"),
     "tp_slabs": (case_tp_slabs, "tp_reduce_push_kernel"),
