@@ -15,13 +15,14 @@
 // few elements), then adds that to a float64 running sum; the CTA's float64
 // partial goes to its own workspace slot, and the slots are added in a fixed
 // order by whoever needs the total: no atomics, the same bits every time.
-// HBM-bound: one read of the gradients. 0.87e9 bf16 gradients: 254 us, 6.9 TB/s
-// (contiguous ranges 259, 16 KB chunks 289).
+// HBM-bound: one read of the gradients. 0.87e9 bf16 gradients: 253-267 us,
+// 6.5-6.9 TB/s, 1.0-1.05 of a copy's rate (contiguous ranges took 2% longer, 16 KB
+// chunks 14%).
 //
 // Clip: the norm kernel, then a kernel whose CTAs each add up the slots (a few
 // KB, from L2) and scale their chunks, last ones first: what the first kernel
-// read last is still in L2. The same gradients: 850 us, of which three passes
-// at the copy rate are 800.
+// read last is still in L2. The same gradients: 857-871 us, in place or not, of
+// which three passes at the copy rate are 800.
 #include "common.cuh"
 
 namespace axon {
@@ -347,9 +348,9 @@ int run_lists(const char* what, const GradLists& g, ClipArgs a, double* part, cu
     return launch_status(what);
   }
   // Gradients that fit L2 (126 MB) are still there for the second pass if its
-  // writes do not push them out: streaming (66 MB: 29 us, 31 without). Of more
-  // than that little is left, and plain accesses are faster (0.8 GB: 393 us, 403
-  // streaming).
+  // writes do not push them out: streaming (66 MB: 7% less time than without). Of
+  // more than that little is left, and plain accesses are faster (0.8 GB: 2.5%
+  // less).
   int64_t bytes = 0;
   for (int64_t i = 0; i < g.count; ++i) bytes += g.n[i] * dtype_size(g.dtype[i]);
   const bool stream = bytes < (126ll << 20);

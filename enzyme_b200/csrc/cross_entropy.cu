@@ -19,7 +19,12 @@
 //             when the target is almost certain, where lse - s_t would cancel.
 //             s_t itself, often the largest logit by far and so the one that
 //             the tensor core's truncating accumulation moves most (4e-5 at
-//             k = 4096), is a dot product of its own in fp32 lanes.
+//             k = 4096), is a dot product of its own in fp32 lanes. The other
+//             words' logits are taken as they are, a sum over k that is cut off
+//             and not rounded at each step: it leaves the loss 1.0e-6 to 1.7e-6
+//             off at k = 4096 (sums in fp32 lanes: 1e-7 to 3e-7). Fewer steps in a
+//             row would mean partial sums that leave tensor memory every few
+//             k-blocks.
 //   kDlogits  a piece of the vocabulary at a time, s is formed again and leaves as
 //             d, rounded to the operand type, in the workspace [rows, piece].
 //             The target's entry is g (p_t - 1) = g expm1(-loss).
@@ -40,7 +45,11 @@
 // epilogues of the products undo it in fp32. So the rounding of d is that of p and
 // p_t - 1, not one that a common g (1 / rows, for the mean) would give every row
 // alike, off by up to half a step of the type in one direction; and in f16
-// probabilities down to 2^-28 keep their digits.
+// probabilities down to 2^-28 keep their digits (in a row of the largest weight: an
+// entry of d is off by up to 2^-39 of that). 16 bits, because the tensor core
+// multiplies d with 16-bit w and h: two terms a value would cost the products a
+// second time. Against 64 bits dh and dw are 0.0019 off (bf16; 0.00025 in f16), where
+// rounding exact results alone is 0.0017 (0.00021).
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -126,7 +135,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// exp(x - ref)
+// exp(x - ref): one ex2.approx, off by 2^-22 of itself and, from its argument's
+// rounding, by 2^-24 of |x - ref|. expf would take several instructions more for
+// each of m x v logits, whose own error is larger.
 __device__ __forceinline__ float exp_from(float x, float ref) { return ex2((x - ref) * kLog2e); }
 
 // mbar_wait by a whole warp, with one answer for all its lanes: where a wait
@@ -544,7 +555,7 @@ __device__ __forceinline__ void dh_tile(const CeParams& p, const Tile& t, uint32
 
 // ---- the CTA-pair kernel ---------------------------------------------------------------
 //
-// Bound by the tensor pipe from some 300 rows up: it is 86-87% active in all three
+// Bound by the tensor pipe from some 300 rows up: it is 85-87% active in the three
 // modes at 2048 x 4096 x 65536, where the loss runs 1549 TFLOP/s, d 1521 and the
 // products 1494 in a burst (cuBLAS here: 1583). At hidden sizes of 512 and less the
 // epilogue shows: 3.1 us a tile at k = 64 (reading 128 KB of tensor memory, the
@@ -725,9 +736,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) ce_pair(const __grid_constant
 //        and neighbouring CTAs write neighbouring pieces of dw's rows. Warps 2
 //        (TMA), 3 (MMA) and 4-11, TMA stores.
 //
-// Gradients in all: 64 rows x 2048 x 32000 94 us (one after the other on CTA
-// pairs 105), one row x 4096 x 128256 591 us (620), where dw written alone takes
-// 3.3 TB/s of the 3.9 and dh alone reads w at 6.4.
+// Gradients in all: 64 rows x 2048 x 32000 94-97 us (one after the other on CTA
+// pairs 105), one row x 4096 x 128256 591-598 us (620), where dw written alone takes
+// 3.3 TB/s of the 3.9 and dh alone reads w at 6.4. Blocks of columns that do not
+// divide the CTAs leave some without dw: 4 of 148 at k = 4096; above k = 18944 each
+// block has one CTA, so 75 at the least write (not measured above 4096).
 constexpr int kFewThreads = 512;
 constexpr int kFewDwStages = 2;                                 // of d transposed, 16 KB
 constexpr int few_h(int few) { return (few + BK - 1) / BK * 2 * B_BYTES; }  // h, 32 KB a k-block
@@ -1018,9 +1031,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) ce_few(const __grid_constant__
 //             and CTA;
 //   kDlogits  a warp's 32 lanes are 32 neighbouring words of a row of d.
 //
-// One row against 128256 words of 4096: 165 us, 6.4 TB/s (0.97 of a copy's rate;
-// the 256-row tiles took 256). 64 rows x 2048 x 32000: 27 us, 4.9 TB/s. 128 rows x
-// 4096 x 128256: 190 us (212).
+// One row against 128256 words of 4096: 170 us as called, ce_stats and all, 6.2 TB/s
+// (0.95 of a copy's rate; the 256-row tiles took 256). 64 rows x 2048 x 32000: 31 us,
+// 4.2 TB/s. 128 rows x 4096 x 128256: 193 us in a burst (212), 223 at a clock that the
+// power cap holds down.
 constexpr int kNarrowRows = 128;
 constexpr int kNarrowMaxStages = 12;
 

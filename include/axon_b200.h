@@ -363,7 +363,9 @@ AXON_API int axon_linear_ce_kept(const void* h, const void* w, const void* targe
  * The logits are formed again, a piece of the vocabulary at a time:
  * tune->split words a piece (a multiple of 256; 0: as many as keep the
  * piece's d, 16-bit [m, piece], within 512 MB). d is rounded to the operand
- * type with dloss scaled to at most 1 (f16: 2^14) and contracted in fp32.
+ * type with dloss scaled to at most 1 (f16: 2^14) and contracted in fp32; f16
+ * rows of far smaller weight than the largest keep fewer digits (an entry of d is
+ * off by up to 2^-39 of the largest |dloss|).
  * workspace: axon_linear_ce_grad_workspace_bytes (same tune), 256-byte aligned,
  * uninitialised. */
 AXON_API int64_t axon_linear_ce_grad_workspace_bytes(int64_t m, int64_t k, int64_t v,
