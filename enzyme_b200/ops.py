@@ -596,17 +596,18 @@ def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", 
     m, k, v, ldh, ldw, bits, red = _head_args("linear_cross_entropy", h, w, targets, reduction, workspace)
     lib, dev = N.lib(), h.device
     with _on_device(dev):
-        # log-sum-exps, the rows' losses, and what is returned as the loss
         each = red == N.AXON_REDUCE_NONE
-        res = torch.empty(2 * m + (m if each else 1), dtype=torch.float32, device=dev)
-        at = res.data_ptr()
+        # tensors of their own, no views of one: each may be changed in place, or be
+        # saved for a backward pass while the other is
+        stats = torch.empty((2, m), dtype=torch.float32, device=dev)
+        loss = torch.empty((m,) if each else (), dtype=torch.float32, device=dev)
+        at, to = stats.data_ptr(), loss.data_ptr()
         ws = _head_workspace(_check_ws_bytes(lib.axon_linear_ce_workspace_bytes(m, k, v)), dev, workspace)
         check(lib.axon_linear_ce_kept(h.data_ptr(), w.data_ptr(), targets.data_ptr(), at, at + 4 * m,
-                                      at + 8 * m if each else None, None if each else at + 8 * m, m, k, v, ldh, ldw,
-                                      dtype_code(h), bits, int(ignore_index), red, ws.data_ptr(), ws.nbytes,
-                                      _tune(tune), _stream(h)))
-    stats = res.as_strided((2, m), (m, 1))
-    return res[2 * m:] if each else res[2 * m], stats
+                                      to if each else None, None if each else to, m, k, v, ldh, ldw, dtype_code(h),
+                                      bits, int(ignore_index), red, ws.data_ptr(), ws.nbytes, _tune(tune),
+                                      _stream(h)))
+    return loss, stats
 
 
 def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100, reduction="mean", need=(True, True),

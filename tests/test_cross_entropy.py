@@ -364,6 +364,20 @@ def test_losses_changed_in_place(m, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_losses_are_no_views(reduction, cuda_device):
+    """Changing the loss in place (weights, accumulation steps) is no change of
+    stats that a backward pass which has saved them would object to."""
+    h, w, t = _inputs(cuda_device, 20, 64, 300, torch.bfloat16, seed=1)
+    loss, stats = ops.linear_cross_entropy(h, w, t, reduction=reduction)
+    assert loss.shape == ((20,) if reduction == "none" else ())
+    before = stats._version
+    loss /= 4
+    assert stats._version == before
+    assert loss.untyped_storage().data_ptr() != stats.untyped_storage().data_ptr()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape,split", [((5, 64, 4160), 4096), ((130, 520, 9000), 8192), ((40, 64, 12345), 0)])
 def test_pieces_whose_contraction_is_cut(shape, split, cuda_device):
     """dh's contraction over a piece in parts, the last piece shorter than the
