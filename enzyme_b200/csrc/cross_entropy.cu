@@ -21,10 +21,12 @@
 //             the tensor core's truncating accumulation moves most (4e-5 at
 //             k = 4096), is a dot product of its own in fp32 lanes. The other
 //             words' logits are taken as they are, a sum over k that is cut off
-//             and not rounded at each step: it leaves the loss 1.0e-6 to 1.7e-6
-//             off at k = 4096 (sums in fp32 lanes: 1e-7 to 3e-7). Fewer steps in a
-//             row would mean partial sums that leave tensor memory every few
-//             k-blocks.
+//             and not rounded at each step: at k = 4096 a row's loss is 9e-7 off,
+//             where a plain fp32 product leaves 7e-7, but all to one side, so the
+//             mean over rows is 1e-6 off (3e-7). Sums over k in two or four parts,
+//             held in registers between them, halved and quartered that and took
+//             2.5% and 4.7% more time (2048 rows; 10% and 12% with 256): not taken.
+//             Up to 64 rows (ce_narrow) such parts cost nothing, and are.
 //   kDlogits  a piece of the vocabulary at a time, s is formed again and leaves as
 //             d, rounded to the operand type, in the workspace [rows, piece].
 //             The target's entry is g (p_t - 1) = g expm1(-loss).
@@ -765,6 +767,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// tmem_wait_ld32 for 16 registers.
+__device__ __forceinline__ void tmem_wait_ld16(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+
 // A tile of dh, transposed: this thread's column (lane) of dh in every row.
 template <typename T>
 __device__ __forceinline__ void few_dh_tile(const CeParams& p, int split, int kb, uint32_t tbase, int64_t col, int lane,
@@ -1052,6 +1063,16 @@ constexpr int narrow_cols(int nt) { return nt < 32 ? nt : 32; }
 constexpr int narrow_epi_warps(int nt) { return 4 * nt / narrow_cols(nt); }
 constexpr int narrow_threads(int nt) { return 64 + 32 * narrow_epi_warps(nt); }
 
+// kLse: the parts that a sum over k is cut into at most, accumulators beside one
+// another (512 columns for two tiles) that the epilogue adds in fp32. The tensor core
+// cuts the sum off at each step and does not round it, always towards zero, so the
+// error grows with the steps: in one part (256 steps at k = 4096) the loss of one row
+// was 1.6e-6 off, in eight it is 1.9e-7 (sums in fp32 lanes: 2.7e-7), in the same
+// time to 1% (reading w bounds it). With more than 64 rows there is room for two
+// parts, which took 2.5% more time and halved 9.5e-7: not taken, as in ce_pair.
+constexpr int narrow_parts(int mode, int nt) { return mode != kLse || nt > 64 ? 1 : nt > 32 ? 4 : 8; }
+constexpr int kPartBlocks = 8;  // k-blocks of a part at least
+
 // Joins (max, sum) pairs.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
   const float mx = fmaxf(a.x, b.x);
@@ -1064,7 +1085,8 @@ __global__ void __launch_bounds__(narrow_threads(NT), 1) ce_narrow(const __grid_
   constexpr int S = narrow_stages(MODE, NT);
   constexpr int SB = narrow_stage(NT);
   constexpr int CW = narrow_cols(NT), EPI = 32 * narrow_epi_warps(NT);
-  constexpr uint32_t COLS = 2 * NT < 32 ? 32 : 2 * NT;
+  constexpr int PARTS = narrow_parts(MODE, NT);
+  constexpr uint32_t COLS = 2 * NT * PARTS < 32 ? 32 : 2 * NT * PARTS;
   static_assert(S * SB >= 129 * NT * 8, "the lanes' pairs are joined in the stages' memory");
   static_assert((2 * S + 5) * 8 + 16 <= 256, "the rows' values begin 256 bytes behind the stages");
   extern __shared__ uint8_t smem_raw[];
@@ -1121,6 +1143,7 @@ __global__ void __launch_bounds__(narrow_threads(NT), 1) ce_narrow(const __grid_
   const int tiles = rows > 0 ? (p.v + p.word_tile - 1) / p.word_tile : 0;
   const uint32_t stage_bytes = static_cast<uint32_t>(p.word_tile * BK * 2 + NT * BK * 2);
   const int kblocks = (p.k + BK - 1) / BK;
+  const int part = PARTS > 1 ? max((kblocks + PARTS - 1) / PARTS, kPartBlocks) : kblocks;
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer ----------------
@@ -1152,19 +1175,23 @@ __global__ void __launch_bounds__(narrow_threads(NT), 1) ce_narrow(const __grid_
       const int buf = i & 1;
       if (!mbar_wait(&tempty[buf], ((i >> 1) & 1) ^ 1u, abort_flag, &g_ce_error)) break;
       tc_fence_after();
-      const uint32_t d = tmem_base + static_cast<uint32_t>(buf * NT);
+      uint32_t d = tmem_base + static_cast<uint32_t>(buf * NT * PARTS);
       bool ok = true;
-      for (int kb = 0; kb < kblocks; ++kb) {
+      for (int kb = 0, left = part; kb < kblocks; ++kb, --left) {
         if (!mbar_wait(&full[stage], phase, abort_flag, &g_ce_error)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        if (left == 0) {  // the next part
+          d += NT;
+          left = part;
+        }
         const uint32_t sa = smem_u32(smem + stage * SB);
         const uint32_t sb = sa + A_BYTES;
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k)
-          tc_mma(d, sdesc(sa + k * 32, 16, 1024), sdesc(sb + k * 32, 16, 1024), id, (kb | k) != 0);
+          tc_mma(d, sdesc(sa + k * 32, 16, 1024), sdesc(sb + k * 32, 16, 1024), id, left != part || k != 0);
         tc_commit(&empty[stage]);
         if (++stage == S) {
           stage = 0;
@@ -1200,14 +1227,24 @@ __global__ void __launch_bounds__(narrow_threads(NT), 1) ce_narrow(const __grid_
       // lanes past the tile's words hold what the stage held before
       const int word = q * 32 + lane < p.word_tile ? t * p.word_tile + q * 32 + lane : 0x7fffffff;
       const uint32_t tbase =
-          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * NT + c0);
+          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * NT * PARTS + c0);
       if (c0 < write) {  // the same for the whole warp
 #pragma unroll
         for (int c1 = 0; c1 < CW; c1 += 16) {
           float v[16];
           __syncwarp();
           tmem_ld16(tbase + c1, v);
-          tmem_wait_ld();
+          tmem_wait_ld16(v);
+          if constexpr (PARTS > 1) {
+#pragma unroll 1
+            for (int at = NT, kb = part; kb < kblocks; at += NT, kb += part) {
+              float u[16];
+              tmem_ld16(tbase + c1 + at, u);
+              tmem_wait_ld16(u);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] += u[j];
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const int c = c1 + j;

@@ -651,6 +651,38 @@ def test_an_almost_certain_target_keeps_its_digits(dtype, m, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,parts", [(1, 8), (16, 8), (20, 8), (60, 4)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_rows_add_k_in_parts(dtype, m, parts, cuda_device):
+    """Up to 64 rows a logit is a sum of parts over k, added in fp32: each part's
+    k / 16 / parts steps are off by at most 2^-23 of the part, as is the module's
+    bound for all of k, and joining them by 2^-24 of the sum each time. Rows that
+    are ignored take every word from there: one word's logit is 7 to 13 with no
+    negative term, the others' are 0. In one part such a logit is 1.0e-4 (bf16)
+    and 2.5e-4 (fp16) off."""
+    k, v = 4096, 1000
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    h = (0.5 + torch.rand(m, k, device=cuda_device, generator=g)).to(dtype)
+    w = torch.zeros(v, k, dtype=dtype, device=cuda_device)
+    w[7] = ((0.5 + torch.rand(k, device=cuda_device, generator=g)) * (10.0 / k)).to(dtype)
+    _, stats = ops.linear_cross_entropy(h, w, torch.full((m,), IGNORE, device=cuda_device), reduction="none")
+    s = h.double() @ w[7].double()
+    want = torch.logaddexp(s, torch.full_like(s, math.log(v - 1)))
+    ds = ((k / 16 / parts + 4) * 2.0 ** -23 + parts * U32) * s
+    assert bool(((stats[0].double() - want).abs() <= ds + E + U32 * want).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [504, 512, 520, 1000, 1032, 2056, 4104, 8200])
+@pytest.mark.parametrize("m", [3, 30, 64])
+def test_few_rows_at_the_ends_of_parts(m, k, cuda_device):
+    """Hidden sizes around one part, around several, and with a short last one."""
+    h, w, t = _inputs(cuda_device, m, k, 700, torch.bfloat16, seed=k, ignored=0.2 if m > 3 else 0.0)
+    _, stats = ops.linear_cross_entropy(h, w, t, reduction="none")
+    Ref(h, w, t).check_loss(stats)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_the_only_word(dtype, cuda_device):
     """A vocabulary of one word: its probability is 1 whatever its logit, so the
