@@ -592,7 +592,10 @@ def linear_cross_entropy(h, w, targets, *, ignore_index=-100, reduction="mean", 
     [0, v) gives NaN. Returns (loss, stats): loss the per-row losses ("none"),
     their sum, or their mean over the rows not ignored, in fp32; stats [2, m]
     fp32 holds each row's log-sum-exp and loss, for linear_cross_entropy_grad.
-    The two share no memory: the losses may be weighted or masked in place."""
+    The two share no memory: the losses may be weighted or masked in place.
+    workspace: a block of memory on h's device, 16-byte aligned, of
+    axon_linear_ce_workspace_bytes; None takes a new one. Calls and captured
+    graphs that may run at once need one each."""
     m, k, v, ldh, ldw, bits, red = _head_args("linear_cross_entropy", h, w, targets, reduction, workspace)
     lib, dev = N.lib(), h.device
     with _on_device(dev):
@@ -619,7 +622,8 @@ def linear_cross_entropy_grad(h, w, targets, stats, dloss, *, ignore_index=-100,
     h's and w's type (dw in fp32 with dw_dtype=torch.float32); need = (True,
     False) or (False, True) leaves one out (None), out = (dh, dw) names the
     tensors to write. Rows that are ignored get zeros. tune={"split": words}
-    sets the piece of the vocabulary that is worked on at a time."""
+    sets the piece of the vocabulary that is worked on at a time. workspace: as
+    for the loss, 256-byte aligned, of axon_linear_ce_grad_workspace_bytes."""
     name = "linear_cross_entropy_grad"
     m, k, v, ldh, ldw, bits, red = _head_args(name, h, w, targets, reduction, workspace)
     lib, dev = N.lib(), h.device
