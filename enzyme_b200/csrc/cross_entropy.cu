@@ -303,13 +303,36 @@ __device__ __forceinline__ float products_scale(const RowHeader* header) {
   return gave_up() ? __int_as_float(0x7fc00000) : header->unscale;
 }
 
+// Waits for this thread's TMEM loads, and ties the 32 registers of one of them to
+// the wait, so that nothing reads them before it.
+__device__ __forceinline__ void tmem_wait_ld32(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+
+// tmem_wait_ld32 for 16 registers.
+__device__ __forceinline__ void tmem_wait_ld16(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+
 // COLS accumulator columns from tensor memory.
 template <int COLS>
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float* v) {
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < COLS; i += 32) tmem_ld32(taddr + i, v + i);
-  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < COLS; i += 32) tmem_wait_ld32(v + i);
 }
 
 __device__ __forceinline__ float max32(const float* v) {
@@ -328,19 +351,6 @@ __device__ __forceinline__ void release_tmem(uint32_t leader_tempty, int lane) {
   tc_fence_before();
   __syncwarp();
   if (lane == 0) mbar_arrive_cluster(leader_tempty, 1);
-}
-
-// Waits for this thread's TMEM loads, and ties the 32 registers of one of them to
-// the wait, so that nothing reads them before it.
-__device__ __forceinline__ void tmem_wait_ld32(float* v) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
-                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
-                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
-                 "+f"(v[30]), "+f"(v[31])
-               :
-               : "memory");
 }
 
 // 32 more words into a row's running maximum and sum; `left` of them count, and
@@ -767,15 +777,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// tmem_wait_ld32 for 16 registers.
-__device__ __forceinline__ void tmem_wait_ld16(float* v) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
-               :
-               : "memory");
-}
-
 // A tile of dh, transposed: this thread's column (lane) of dh in every row.
 template <typename T>
 __device__ __forceinline__ void few_dh_tile(const CeParams& p, int split, int kb, uint32_t tbase, int64_t col, int lane,
@@ -787,7 +788,7 @@ __device__ __forceinline__ void few_dh_tile(const CeParams& p, int split, int kb
     float v[16];
     __syncwarp();
     tmem_ld16(tbase + r, v);
-    tmem_wait_ld();
+    tmem_wait_ld16(v);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       if (!ok || r + j >= rows) continue;
